@@ -443,3 +443,201 @@ def quantize_per_token_int8(x, q, scale, rows, k, x_type=DTYPE_F32, x_pitch=0, s
     args = QuantizeInt8Args(rows=rows, k=k, x_type=x_type, reserved=0, x_pitch=x_pitch, x=_p(x), q=_p(q), scale=_p(scale))
     _check("cb200_quantize_per_token_int8", load().cb200_quantize_per_token_int8(ctypes.byref(args), _stream(stream)))
 
+
+
+# ---- routing, dispatch, combine and the NVFP4 format
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+ROUTE_GROUP_MAX, ROUTE_GROUP_TOP2_SUM = 0, 1
+ROUTE_RENORMALIZE = 1
+DISPATCH_INDEX, DISPATCH_COPY, DISPATCH_INT8, DISPATCH_MX_E4M3, DISPATCH_NVFP4 = 0, 1, 2, 3, 4
+NVFP4_SCALES_ROWS, NVFP4_SCALES_TILED = 0, 1
+NVFP4_SWIGLU = 1
+_FLOAT_BYTES = {DTYPE_F32: 4, DTYPE_BF16: 2, DTYPE_F16: 2}
+
+
+class MoeRouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _u32), ("experts", _u32), ("top_k", _u32), ("score", _u32), ("groups", _u32), ("groups_kept", _u32),
+        ("group_score", _u32), ("flags", _u32), ("logits_type", _u32), ("scaling", ctypes.c_float),
+        ("logits_pitch", _u64), ("logits", _vp), ("bias", _vp), ("token_count", _vp), ("weights", _vp), ("ids", _vp),
+    ]
+
+
+class MoeDispatchArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _u32), ("experts", _u32), ("top_k", _u32), ("k", _u32), ("format", _u32), ("x_type", _u32),
+        ("expert_begin", ctypes.c_int32), ("group_list_type", _u32), ("group_list_kind", _u32),
+        ("row_index_type", _u32), ("x_pitch", _u64), ("x", _vp), ("ids", _vp), ("weights", _vp), ("tensor_scale", _vp),
+        ("q", _vp), ("scale", _vp), ("group_list", _vp), ("position", _vp), ("row_index", _vp), ("row_weight", _vp),
+        ("workspace", _vp), ("workspace_bytes", _u64),
+    ]
+
+
+class MoeCombineArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _u32), ("top_k", _u32), ("n", _u32), ("rows", _u32), ("d_type", _u32), ("out_type", _u32),
+        ("shared_weight", ctypes.c_float), ("reserved", _u32), ("d", _vp), ("position", _vp), ("weights", _vp),
+        ("shared", _vp), ("out", _vp),
+    ]
+
+
+class Nvfp4QuantizeArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _u32), ("k", _u32), ("x_type", _u32), ("scale_layout", _u32), ("flags", _u32),
+        ("row_count_type", _u32), ("x_pitch", _u64), ("x", _vp), ("tensor_scale", _vp), ("row_count", _vp), ("q", _vp),
+        ("scale", _vp),
+    ]
+
+
+_prepared = {}
+
+
+def _function(name, args_t, result=ctypes.c_int):
+    """The library's function `name` with its argument types set (looked up once)."""
+    fn = _prepared.get(name)
+    if fn is None:
+        fn = getattr(load(), name)
+        fn.argtypes = [ctypes.POINTER(args_t)] + ([_vp] if result is ctypes.c_int and not name.endswith("_can_implement") else [])
+        fn.restype = result
+        _prepared[name] = fn
+    return fn
+
+
+def _buffer(t, nbytes, what, like=None):
+    """Address of a CUDA tensor used as a raw buffer of at least `nbytes` bytes; None stays None."""
+    if t is None:
+        return None
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous CUDA tensor")
+    if t.nbytes < nbytes:
+        raise ValueError(f"{what} holds {t.nbytes} bytes, {nbytes} are needed")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{what} is on another device")
+    return t.data_ptr()
+
+
+def _rows(t, rows, width, pitch, elem, what, like=None):
+    """As _buffer, for `rows` rows of `width` elements with `pitch` elements between them (a view with strided rows is
+    taken: only the storage behind its first element has to be long enough)."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    need = ((rows - 1) * (pitch or width) + width) * elem if rows and width else 0
+    have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+    if have < need:
+        raise ValueError(f"{what} holds {have} bytes, {need} are needed")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{what} is on another device")
+    return t.data_ptr()
+
+
+def _enqueue(name, args, like, stream):
+    """Calls the library on the device of `like`, on `stream` or that device's current stream."""
+    import torch
+    fn = _function(name, type(args))
+    device = like.get_device()
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    if torch.cuda.current_device() == device:
+        _check(name, fn(ctypes.byref(args), stream.cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            _check(name, fn(ctypes.byref(args), stream.cuda_stream))
+
+
+def _float_bytes(type_code, what):
+    if type_code not in _FLOAT_BYTES:
+        raise ValueError(f"{what} must be DTYPE_F32, DTYPE_BF16 or DTYPE_F16")
+    return _FLOAT_BYTES[type_code]
+
+
+def moe_route(logits, weights, ids, tokens, experts, top_k, score=ROUTE_SOFTMAX, bias=None, groups=1, groups_kept=None,
+              group_score=ROUTE_GROUP_MAX, renormalize=True, scaling=1.0, logits_type=DTYPE_F32, logits_pitch=0,
+              token_count=None, stream=None):
+    """logits [tokens][experts] -> weights fp32 and ids int32 [tokens][top_k], the experts with the largest scores (plus
+    bias) of the best groups, ties to the lower index; id -1 and weight 0 where no expert is left."""
+    out = tokens * top_k * 4
+    args = MoeRouteArgs(tokens, experts, top_k, score, groups, groups if groups_kept is None else groups_kept,
+                        group_score, ROUTE_RENORMALIZE if renormalize else 0, logits_type, scaling, logits_pitch,
+                        _rows(logits, tokens, experts, logits_pitch, _float_bytes(logits_type, "logits_type"), "logits"),
+                        _buffer(bias, experts * 4, "bias", logits), _buffer(token_count, 4, "token_count", logits),
+                        _buffer(weights, out, "weights", logits), _buffer(ids, out, "ids", logits))
+    _enqueue("cb200_moe_route", args, logits, stream)
+
+
+def moe_dispatch_workspace_size(tokens, experts, top_k):
+    args = MoeDispatchArgs(tokens=tokens, experts=experts, top_k=top_k, format=DISPATCH_INDEX, ids=256, position=256,
+                           group_list=256)
+    return int(_function("cb200_moe_dispatch_workspace_size", MoeDispatchArgs, _u64)(ctypes.byref(args)))
+
+
+def _dispatch_sizes(rows, k, fmt, x_bytes):
+    """Bytes of q and of scale that `rows` dispatched rows take."""
+    if fmt == DISPATCH_COPY:
+        return rows * k * x_bytes, 0
+    if fmt == DISPATCH_INT8:
+        return rows * k, rows * 4
+    if fmt == DISPATCH_MX_E4M3:
+        return rows * k, rows * ((k // 32 + 1) // 2 * 2)
+    if fmt == DISPATCH_NVFP4:
+        return rows * (k // 2), rows * (k // 16)
+    return 0, 0
+
+
+def moe_dispatch(x, ids, weights, group_list, position, tokens, experts, top_k, k, fmt, q=None, scale=None,
+                 row_index=None, row_weight=None, x_type=DTYPE_BF16, x_pitch=0, tensor_scale=None, workspace=None,
+                 expert_begin=0, group_list_type=GROUP_LIST_INT64, group_list_kind=GROUP_LIST_PREFIX_SUMS,
+                 row_index_type=GROUP_LIST_INT32, stream=None):
+    """ids, weights [tokens][top_k] of a router -> rows sorted by expert: group_list [experts], position [tokens][top_k]
+    (row of each pair, -1 when dropped), row_index / row_weight [tokens * top_k], and x [tokens][k] written to its rows
+    of q / scale in the format `fmt`.  workspace: moe_dispatch_workspace_size bytes."""
+    rows = tokens * top_k
+    x_bytes = _float_bytes(x_type, "x_type")
+    q_bytes, scale_bytes = _dispatch_sizes(rows, k, fmt, x_bytes)
+    index_bytes = 8 if row_index_type == GROUP_LIST_INT64 else 4
+    args = MoeDispatchArgs(
+        tokens, experts, top_k, k, fmt, x_type, expert_begin, group_list_type, group_list_kind, row_index_type, x_pitch,
+        None if fmt == DISPATCH_INDEX else _rows(x, tokens, k, x_pitch, x_bytes, "x", ids),
+        _buffer(ids, rows * 4, "ids"), _buffer(weights, rows * 4, "weights", ids),
+        _buffer(tensor_scale, 4, "tensor_scale", ids), _buffer(q, q_bytes, "q", ids),
+        _buffer(scale, scale_bytes, "scale", ids),
+        _buffer(group_list, experts * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", ids),
+        _buffer(position, rows * 4, "position", ids), _buffer(row_index, rows * index_bytes, "row_index", ids),
+        _buffer(row_weight, rows * 4, "row_weight", ids), _buffer(workspace, 0, "workspace", ids),
+        0 if workspace is None else workspace.nbytes)
+    _enqueue("cb200_moe_dispatch", args, ids, stream)
+
+
+def moe_combine(d, position, weights, out, tokens, n, top_k, rows=None, d_type=DTYPE_BF16, out_type=DTYPE_BF16,
+                shared=None, shared_weight=1.0, stream=None):
+    """out[t] = shared_weight * shared[t] + sum_j weights[t][j] * d[position[t][j]], d [rows][n] (rows: tokens * top_k
+    unless given), slots with a negative position skipped."""
+    rows = tokens * top_k if rows is None else rows
+    out_bytes = tokens * n * _float_bytes(out_type, "out_type")
+    args = MoeCombineArgs(tokens, top_k, n, rows, d_type, out_type, shared_weight, 0,
+                          _buffer(d, rows * n * _float_bytes(d_type, "d_type"), "d"),
+                          _buffer(position, tokens * top_k * 4, "position", d),
+                          _buffer(weights, tokens * top_k * 4, "weights", d), _buffer(shared, out_bytes, "shared", d),
+                          _buffer(out, out_bytes, "out", d))
+    _enqueue("cb200_moe_combine", args, d, stream)
+
+
+def nvfp4_tiled_scale_bytes(rows, k):
+    """Bytes of a tiled scale array of rows x k elements."""
+    return (rows + 127) // 128 * ((k + 63) // 64) * 512
+
+
+def nvfp4_quantize(x, q, scale, rows, k, tensor_scale, x_type=DTYPE_BF16, x_pitch=0, scale_layout=NVFP4_SCALES_ROWS,
+                   swiglu=False, row_count=None, row_count_type=GROUP_LIST_INT64, stream=None):
+    """x [rows][k] (with swiglu [rows][2k]: act next to gate) -> q [rows][k/2] bytes and E4M3 scales by rows ([rows][k/16]
+    bytes) or tiled (nvfp4_tiled_scale_bytes bytes), in units of the device scalar tensor_scale."""
+    width = 2 * k if swiglu else k
+    scale_bytes = nvfp4_tiled_scale_bytes(rows, k) if scale_layout == NVFP4_SCALES_TILED else rows * (k // 16)
+    args = Nvfp4QuantizeArgs(
+        rows, k, x_type, scale_layout, NVFP4_SWIGLU if swiglu else 0, row_count_type, x_pitch,
+        _rows(x, rows, width, x_pitch, _float_bytes(x_type, "x_type"), "x"),
+        _buffer(tensor_scale, 4, "tensor_scale", x),
+        _buffer(row_count, 8 if row_count_type == GROUP_LIST_INT64 else 4, "row_count", x),
+        _buffer(q, rows * (k // 2), "q", x), _buffer(scale, scale_bytes, "scale", x))
+    _enqueue("cb200_nvfp4_quantize", args, x, stream)

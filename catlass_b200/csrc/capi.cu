@@ -18,6 +18,10 @@
 #include "routing.cuh"
 #include "ingest.cuh"
 #include "mx_quantize.cuh"
+#include "moe_route.cuh"
+#include "moe_combine.cuh"
+#include "nvfp4_quantize.cuh"
+#include "moe_dispatch.cuh"
 
 using namespace cb200;
 using namespace cb200::host;
@@ -2362,6 +2366,8 @@ int cb200_mx_quantize(const cb200_mx_quantize_args* args, void* stream_v)
 }
 
 }  // extern "C"
+
+#include "capi_moe.cuh"
 
 #ifdef CB200_DEVELOPER_KNOBS
 // Developer builds only: reads and clears the W4A8 kernel's per-role cycle counters.

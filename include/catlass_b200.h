@@ -575,6 +575,177 @@ typedef struct cb200_quantize_int8_args {
 CB200_API int cb200_quantize_per_token_int8_can_implement(const cb200_quantize_int8_args *args);
 CB200_API int cb200_quantize_per_token_int8(const cb200_quantize_int8_args *args, void *stream);
 
+/*
+ * Routing of tokens to experts (the step in front of a grouped matmul): per token t, with logits x[t][0 .. experts),
+ *     s[e]   = exp(x[e]) / sum exp(x)      (CB200_ROUTE_SOFTMAX)    or   1 / (1 + exp(-x[e]))   (CB200_ROUTE_SIGMOID)
+ *     key[e] = s[e] + bias[e];  without a bias the order of s, which is the order of x
+ *     groups > 1: the experts lie in `groups` equal runs; a run's key is its largest key (CB200_ROUTE_GROUP_MAX) or the
+ *              sum of its two largest (CB200_ROUTE_GROUP_TOP2_SUM; without a bias, of its two largest s); only experts of
+ *              the `groups_kept` runs with the largest keys can be chosen
+ *     ids[t] = the top_k experts by key, largest first;  weights[t][j] = s[ids[t][j]], divided by their sum over j with
+ *              CB200_ROUTE_RENORMALIZE (a sum of zero gives zeros), times `scaling`
+ * Ties, of experts and of runs, go to the lower index.  The order is that of the exact keys: where two keys are closer
+ * than 32-bit arithmetic can tell apart, they are worked out again in 64 bits.
+ * An expert whose logit is -inf or NaN cannot be chosen and has s = 0; slots left without an expert get id -1 and
+ * weight 0, which cb200_moe_dispatch and cb200_moe_combine skip.  Logits of +inf share the softmax among themselves.
+ * token_count (optional, device, int32): tokens at or beyond it (a padded batch) get ids -1 and weights 0.
+ * The reference has no router; its finalize-routing example makes logit and row_index on the host
+ * (experimental/gmm/ascend950_fp8_mx_grouped_matmul_finalize_routing/gen_data_compare.py).  No workspace.
+ */
+#define CB200_ROUTE_SOFTMAX 0
+#define CB200_ROUTE_SIGMOID 1
+#define CB200_ROUTE_GROUP_MAX 0
+#define CB200_ROUTE_GROUP_TOP2_SUM 1
+#define CB200_ROUTE_RENORMALIZE 1u
+typedef struct cb200_moe_route_args {
+    uint32_t tokens;
+    uint32_t experts;       /* 1 .. 1024 */
+    uint32_t top_k;         /* 1 .. 32, at most the experts of groups_kept groups */
+    uint32_t score;         /* CB200_ROUTE_SOFTMAX / _SIGMOID */
+    uint32_t groups;        /* 1 .. 32, divides experts */
+    uint32_t groups_kept;   /* 1 .. groups */
+    uint32_t group_score;   /* CB200_ROUTE_GROUP_MAX / _TOP2_SUM */
+    uint32_t flags;         /* 0 or CB200_ROUTE_RENORMALIZE */
+    uint32_t logits_type;   /* CB200_DTYPE_F32, _BF16 or _F16 */
+    float scaling;
+    uint64_t logits_pitch;  /* elements between tokens; 0 = experts */
+    const void *logits;     /* [tokens][experts] */
+    const float *bias;      /* [experts] finite, or NULL */
+    const int32_t *token_count;
+    float *weights;         /* out [tokens][top_k] */
+    int32_t *ids;           /* out [tokens][top_k] */
+} cb200_moe_route_args;
+
+CB200_API int cb200_moe_route_can_implement(const cb200_moe_route_args *args);
+CB200_API int cb200_moe_route(const cb200_moe_route_args *args, void *stream);
+
+/*
+ * Dispatch of routed tokens: sorts the (token, slot) pairs by expert, and writes every token's activations, quantised
+ * once, to its rows: exactly what the grouped matmuls read.
+ *     pair p = t * top_k + j goes to expert ids[p] - expert_begin; pairs outside [0, experts) are dropped
+ *     rows are sorted by expert, inside an expert by p (the same order on every run)
+ *     position[p]    row of pair p, -1 when dropped
+ *     row_index[r]   token of row r;      row_weight[r]  weights of the pair of row r
+ *     group_list     row counts of the experts or ascending prefix sums, int64 or int32
+ *     q, scale       row r holds x[row_index[r]] in the format asked for:
+ *         CB200_DISPATCH_INDEX     nothing (x, q and scale are not read)
+ *         CB200_DISPATCH_COPY      the row as it is, in x's type                                (no scale)
+ *         CB200_DISPATCH_INT8      as cb200_quantize_per_token_int8: q [rows][k], scale fp32 [rows]
+ *         CB200_DISPATCH_MX_E4M3   as cb200_mx_quantize: q [rows][k], scale E8M0 [rows][KS]
+ *         CB200_DISPATCH_NVFP4     as cb200_nvfp4_quantize with tensor_scale, scales by rows: q [rows][k/2], scale [rows][k/16]
+ * row_index (int32 or int64), row_weight and position are what cb200_mx_grouped_matmul_finalize_routing and
+ * cb200_moe_combine read.  The outputs hold tokens * top_k rows; rows past the last expert's are left as they were.
+ * Requirements: x, its rows (x_pitch) and q 16-byte aligned, k a multiple of 16 (INT8, NVFP4) or 32 (MX_E4M3), or of 16
+ * bytes (COPY); tokens * top_k < 2^24.  The workspace (cb200_moe_dispatch_workspace_size bytes, 256-byte aligned)
+ * holds counts.  The reference has no such kernel: its examples sort and quantise on the host.
+ */
+#define CB200_DISPATCH_INDEX 0
+#define CB200_DISPATCH_COPY 1
+#define CB200_DISPATCH_INT8 2
+#define CB200_DISPATCH_MX_E4M3 3
+#define CB200_DISPATCH_NVFP4 4
+typedef struct cb200_moe_dispatch_args {
+    uint32_t tokens;
+    uint32_t experts;             /* 1 .. 1024 (the group count of the matmul that follows) */
+    uint32_t top_k;               /* 1 .. 32 */
+    uint32_t k;                   /* elements of a token's row */
+    uint32_t format;              /* CB200_DISPATCH_* */
+    uint32_t x_type;              /* CB200_DTYPE_F32, _BF16 or _F16 */
+    int32_t expert_begin;         /* id of the first of the `experts` experts (expert-sharded ranks) */
+    uint32_t group_list_type;     /* CB200_GROUP_LIST_INT64 / _INT32 */
+    uint32_t group_list_kind;     /* CB200_GROUP_LIST_SIZES / CB200_GROUP_LIST_PREFIX_SUMS */
+    uint32_t row_index_type;      /* CB200_GROUP_LIST_INT64 / _INT32 */
+    uint64_t x_pitch;             /* elements between tokens of x; 0 = k */
+    const void *x;                /* [tokens][k] */
+    const int32_t *ids;           /* [tokens][top_k] */
+    const float *weights;         /* [tokens][top_k]; may be NULL when row_weight is */
+    const float *tensor_scale;    /* device scalar, NVFP4 only */
+    void *q;
+    void *scale;
+    void *group_list;             /* out [experts] */
+    int32_t *position;            /* out [tokens][top_k] */
+    void *row_index;              /* out [tokens * top_k], or NULL */
+    float *row_weight;            /* out [tokens * top_k], or NULL */
+    void *workspace;
+    uint64_t workspace_bytes;
+} cb200_moe_dispatch_args;
+
+CB200_API int cb200_moe_dispatch_can_implement(const cb200_moe_dispatch_args *args);
+CB200_API uint64_t cb200_moe_dispatch_workspace_size(const cb200_moe_dispatch_args *args);
+CB200_API int cb200_moe_dispatch(const cb200_moe_dispatch_args *args, void *stream);
+
+/*
+ * Combine: the weighted sum of a token's expert rows, for grouped matmuls that write D row by row (W8A8, MX, NVFP4;
+ * cb200_mx_grouped_matmul_finalize_routing has it fused):
+ *     out[t] = round( shared_weight * shared[t] + sum_j weights[t][j] * d[position[t][j]] )       fp32, j ascending
+ * Slots with position < 0 or >= rows are skipped (their weight is not read into the sum); shared may be NULL.  Every
+ * row of out is written, with the same bits on every run.  No workspace.
+ */
+typedef struct cb200_moe_combine_args {
+    uint32_t tokens;
+    uint32_t top_k;               /* 1 .. 32 */
+    uint32_t n;
+    uint32_t rows;                /* rows of d */
+    uint32_t d_type;              /* CB200_DTYPE_F32, _BF16 or _F16 */
+    uint32_t out_type;            /* CB200_DTYPE_F32, _BF16 or _F16; shared has this type too */
+    float shared_weight;
+    uint32_t reserved;            /* 0 */
+    const void *d;                /* [rows][n] */
+    const int32_t *position;      /* [tokens][top_k] */
+    const float *weights;         /* [tokens][top_k] */
+    const void *shared;           /* [tokens][n] or NULL */
+    void *out;                    /* [tokens][n] */
+} cb200_moe_combine_args;
+
+CB200_API int cb200_moe_combine_can_implement(const cb200_moe_combine_args *args);
+CB200_API int cb200_moe_combine(const cb200_moe_combine_args *args, void *stream);
+
+/*
+ * NVFP4: 4-bit floating point (E2M1) with one E4M3 scale per 16 elements along k and one fp32 scale per tensor; the
+ * block is half of MXFP4's and its scale has a mantissa, so a block's largest element lands on 6 instead of
+ * somewhere in (3, 6].  A value is  code * scale * tensor_scale.
+ *
+ * cb200_nvfp4_quantize: x (rows x k, row pitch x_pitch elements) -> q [rows][k/2] bytes (even index in bits 0-3) and
+ * E4M3 scales.  Per block, each step in fp32:
+ *     scale = e4m3( min(448, amax / (6 * tensor_scale)) )      nearest, ties to even
+ *     q[i]  = e2m1( x[i] * (1 / (scale * tensor_scale)) )      nearest, ties to the even code, at most 6
+ * A block whose scale rounds to zero (or whose 1 / (scale * tensor_scale) is not finite) gets codes 0; a block that holds
+ * Inf or NaN gets a NaN scale (0x7F) and codes 0, so that the products it enters are NaN.
+ * With CB200_NVFP4_SWIGLU x has 2k columns and the value is  act / (1 + exp(-act)) * gate  with act = x[:, :k] and
+ * gate = x[:, k:]: the step between the two matmuls of an expert.
+ * Scale layouts:
+ *     CB200_NVFP4_SCALES_ROWS   [rows][k/16] bytes
+ *     CB200_NVFP4_SCALES_TILED  [ceil(rows/128)][ceil(k/64)][32][4][4] bytes: the scale of row r and block b is at
+ *                               [r / 128][b / 4][r % 32][r % 128 / 32][b % 4], what the tensor core reads without a
+ *                               rewrite.  Bytes of blocks past k/16 must be 0 (the quantiser writes them); bytes of
+ *                               rows past the last are not used and not written.
+ * row_count (optional, device, int32 or int64 as row_count_type): rows at or beyond it are left as they were.  With
+ * the last entry of a prefix-sum group list only the rows that a dispatch filled are worked on.
+ * Requirements: k a multiple of 16; x and its rows 16-byte aligned (with SWIGLU both halves), q 8-byte aligned.
+ */
+#define CB200_NVFP4_SCALES_ROWS 0
+#define CB200_NVFP4_SCALES_TILED 1
+#define CB200_NVFP4_SWIGLU 1u
+typedef struct cb200_nvfp4_quantize_args {
+    uint32_t rows, k;
+    uint32_t x_type;              /* CB200_DTYPE_F32, _BF16 or _F16 */
+    uint32_t scale_layout;        /* CB200_NVFP4_SCALES_ROWS / _TILED */
+    uint32_t flags;               /* 0 or CB200_NVFP4_SWIGLU */
+    uint32_t row_count_type;      /* CB200_GROUP_LIST_INT64 / _INT32 */
+    uint64_t x_pitch;             /* elements between rows of x; 0 = k, or 2k with CB200_NVFP4_SWIGLU */
+    const void *x;
+    const float *tensor_scale;    /* device scalar, > 0 */
+    const void *row_count;        /* device scalar or NULL */
+    void *q;
+    void *scale;
+} cb200_nvfp4_quantize_args;
+
+CB200_API int cb200_nvfp4_quantize_can_implement(const cb200_nvfp4_quantize_args *args);
+CB200_API int cb200_nvfp4_quantize(const cb200_nvfp4_quantize_args *args, void *stream);
+
+/* Bytes of a tiled scale array of rows x k elements. */
+CB200_API uint64_t cb200_nvfp4_tiled_scale_bytes(uint32_t rows, uint32_t k);
+
 /* ---- library / device state ---- */
 
 /* Reads and clears the status word kernels of this library write on the current device when a bounded
