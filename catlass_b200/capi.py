@@ -489,6 +489,23 @@ class Nvfp4QuantizeArgs(ctypes.Structure):
     ]
 
 
+class Nvfp4MatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", _u32), ("n", _u32), ("k", _u32), ("scale_a_layout", _u32), ("scale_b_layout", _u32), ("d_type", _u32),
+        ("a", _vp), ("b", _vp), ("scale_a", _vp), ("scale_b", _vp), ("alpha", _vp), ("d", _vp), ("workspace", _vp),
+        ("workspace_bytes", _u64), ("block_num", _u32), ("flags", _u32),
+    ]
+
+
+class Nvfp4GroupedMatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", _u32), ("n", _u32), ("k", _u32), ("group_count", _u32), ("scale_b_layout", _u32), ("group_list_type", _u32),
+        ("group_list_kind", _u32), ("d_type", _u32), ("a", _vp), ("b", _vp), ("group_list", _vp), ("scale_a", _vp),
+        ("scale_b", _vp), ("alpha", _vp), ("d", _vp), ("workspace", _vp), ("workspace_bytes", _u64), ("block_num", _u32),
+        ("flags", _u32),
+    ]
+
+
 _prepared = {}
 
 
@@ -641,3 +658,49 @@ def nvfp4_quantize(x, q, scale, rows, k, tensor_scale, x_type=DTYPE_BF16, x_pitc
         _buffer(row_count, 8 if row_count_type == GROUP_LIST_INT64 else 4, "row_count", x),
         _buffer(q, rows * (k // 2), "q", x), _buffer(scale, scale_bytes, "scale", x))
     _enqueue("cb200_nvfp4_quantize", args, x, stream)
+
+
+def _nvfp4_scale_bytes(rows, k, layout):
+    return nvfp4_tiled_scale_bytes(rows, k) if layout == NVFP4_SCALES_TILED else rows * (k // 16)
+
+
+def nvfp4_matmul_workspace_size(m, n, k, scale_a_layout=NVFP4_SCALES_ROWS, scale_b_layout=NVFP4_SCALES_ROWS):
+    args = Nvfp4MatmulArgs(m=m, n=n, k=k, scale_a_layout=scale_a_layout, scale_b_layout=scale_b_layout, a=256, b=256,
+                           scale_a=256, scale_b=256, d=256)
+    return int(_function("cb200_nvfp4_matmul_workspace_size", Nvfp4MatmulArgs, _u64)(ctypes.byref(args)))
+
+
+def nvfp4_matmul(a, b, scale_a, scale_b, d, m, n, k, workspace=None, alpha=None, scale_a_layout=NVFP4_SCALES_ROWS,
+                 scale_b_layout=NVFP4_SCALES_ROWS, d_type=DTYPE_BF16, stream=None, block_num=0):
+    """a [m][k/2], b [n][k/2] packed E2M1 with E4M3 scales by rows or tiled -> d [m][n] = alpha * a @ b^T.  alpha: device
+    scalar (the product of the tensor scales); workspace: nvfp4_matmul_workspace_size bytes."""
+    args = Nvfp4MatmulArgs(
+        m, n, k, scale_a_layout, scale_b_layout, d_type, _buffer(a, m * (k // 2), "a"), _buffer(b, n * (k // 2), "b", a),
+        _buffer(scale_a, _nvfp4_scale_bytes(m, k, scale_a_layout), "scale_a", a),
+        _buffer(scale_b, _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", a), _buffer(alpha, 4, "alpha", a),
+        _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", a), _buffer(workspace, 0, "workspace", a),
+        0 if workspace is None else workspace.nbytes, block_num, 0)
+    _enqueue("cb200_nvfp4_matmul", args, a, stream)
+
+
+def nvfp4_grouped_matmul_workspace_size(m, n, k, group_count, scale_b_layout=NVFP4_SCALES_ROWS):
+    args = Nvfp4GroupedMatmulArgs(m=m, n=n, k=k, group_count=group_count, scale_b_layout=scale_b_layout, a=256, b=256,
+                                  group_list=256, scale_a=256, scale_b=256, d=256)
+    return int(_function("cb200_nvfp4_grouped_matmul_slice_m_workspace_size", Nvfp4GroupedMatmulArgs, _u64)(
+        ctypes.byref(args)))
+
+
+def nvfp4_grouped_matmul(a, b, group_list, scale_a, scale_b, d, m, n, k, group_count, workspace, alpha=None,
+                         scale_b_layout=NVFP4_SCALES_ROWS, d_type=DTYPE_BF16, group_list_type=GROUP_LIST_INT64,
+                         group_list_kind=GROUP_LIST_SIZES, stream=None, block_num=0):
+    """Grouped slice-M NVFP4 matmul: a [m][k/2], b [G][n][k/2], scale_a by rows, scale_b by rows or tiled per group,
+    alpha [G] on the device; rows past the last group are not written."""
+    args = Nvfp4GroupedMatmulArgs(
+        m, n, k, group_count, scale_b_layout, group_list_type, group_list_kind, d_type, _buffer(a, m * (k // 2), "a"),
+        _buffer(b, group_count * n * (k // 2), "b", a),
+        _buffer(group_list, group_count * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", a),
+        _buffer(scale_a, m * (k // 16), "scale_a", a),
+        _buffer(scale_b, group_count * _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", a),
+        _buffer(alpha, group_count * 4, "alpha", a), _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", a),
+        _buffer(workspace, 0, "workspace", a), 0 if workspace is None else workspace.nbytes, block_num, 0)
+    _enqueue("cb200_nvfp4_grouped_matmul_slice_m", args, a, stream)

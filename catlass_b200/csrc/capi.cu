@@ -21,6 +21,8 @@
 #include "moe_route.cuh"
 #include "moe_combine.cuh"
 #include "nvfp4_quantize.cuh"
+#include "nvfp4_gemm.cuh"
+#include "nvfp4_few.cuh"
 #include "moe_dispatch.cuh"
 
 using namespace cb200;
@@ -2368,6 +2370,7 @@ int cb200_mx_quantize(const cb200_mx_quantize_args* args, void* stream_v)
 }  // extern "C"
 
 #include "capi_moe.cuh"
+#include "capi_nvfp4.cuh"
 
 #ifdef CB200_DEVELOPER_KNOBS
 // Developer builds only: reads and clears the W4A8 kernel's per-role cycle counters.

@@ -746,6 +746,69 @@ CB200_API int cb200_nvfp4_quantize(const cb200_nvfp4_quantize_args *args, void *
 /* Bytes of a tiled scale array of rows x k elements. */
 CB200_API uint64_t cb200_nvfp4_tiled_scale_bytes(uint32_t rows, uint32_t k);
 
+/*
+ * NVFP4 matmul:  D[i,j] = round( alpha * sum_k (A[i,k] * scale_a[i,k/16]) * (B[k,j] * scale_b[j,k/16]) ), fp32 sums
+ *     a  [m][k/2] bytes      b  [n][k/2] bytes (column-major B)      d  [m][n] bf16, fp16 or fp32
+ * alpha: device scalar, the product of the two tensor scales, or NULL for 1.
+ * Requirements: k a multiple of 32; a, b, the scales and the workspace 16-byte aligned (the workspace 256).
+ * Scales that come by rows are re-tiled into the workspace first (cb200_nvfp4_matmul_workspace_size bytes, 0 when both
+ * are tiled): one extra pass over them.  Keep the weights' scales tiled.
+ * The fp32 sums are those of the tensor core over K, in chunks of 64; few rows of A may split K over the CTAs of a
+ * cluster, whose partial sums are added in a fixed order.  The same call gives the same bits on every run.
+ */
+typedef struct cb200_nvfp4_matmul_args {
+    uint32_t m, n, k;
+    uint32_t scale_a_layout;      /* CB200_NVFP4_SCALES_ROWS / _TILED */
+    uint32_t scale_b_layout;      /* CB200_NVFP4_SCALES_ROWS / _TILED */
+    uint32_t d_type;              /* CB200_DTYPE_BF16, _F16 or _F32 */
+    const void *a;
+    const void *b;
+    const void *scale_a;
+    const void *scale_b;
+    const float *alpha;
+    void *d;
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint32_t block_num;           /* upper bound on the CTAs launched; 0 = one per SM */
+    uint32_t flags;               /* 0 */
+} cb200_nvfp4_matmul_args;
+
+CB200_API int cb200_nvfp4_matmul_can_implement(const cb200_nvfp4_matmul_args *args);
+CB200_API uint64_t cb200_nvfp4_matmul_workspace_size(const cb200_nvfp4_matmul_args *args);
+CB200_API int cb200_nvfp4_matmul(const cb200_nvfp4_matmul_args *args, void *stream);
+
+/*
+ * Grouped (slice-M) NVFP4 matmul: group g owns a run of rows of A and D, its own weight matrix b[g] [n][k/2], its
+ * scales and alpha[g].  group_list as for cb200_mx_grouped_matmul_slice_m (row counts or prefix sums, clamped to m;
+ * rows past the last group are not written).
+ *     scale_a  by rows, [m][k/16]
+ *     scale_b  by rows [group_count][n][k/16], or tiled, one tiled array of n x k per group
+ *     alpha    device [group_count], or NULL for 1
+ */
+typedef struct cb200_nvfp4_grouped_matmul_args {
+    uint32_t m, n, k;
+    uint32_t group_count;         /* 1 .. 1024 */
+    uint32_t scale_b_layout;      /* CB200_NVFP4_SCALES_ROWS / _TILED */
+    uint32_t group_list_type;     /* CB200_GROUP_LIST_INT64 / _INT32 */
+    uint32_t group_list_kind;     /* CB200_GROUP_LIST_SIZES / CB200_GROUP_LIST_PREFIX_SUMS */
+    uint32_t d_type;              /* CB200_DTYPE_BF16, _F16 or _F32 */
+    const void *a;
+    const void *b;
+    const void *group_list;
+    const void *scale_a;
+    const void *scale_b;
+    const float *alpha;
+    void *d;
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint32_t block_num;
+    uint32_t flags;               /* 0 */
+} cb200_nvfp4_grouped_matmul_args;
+
+CB200_API int cb200_nvfp4_grouped_matmul_slice_m_can_implement(const cb200_nvfp4_grouped_matmul_args *args);
+CB200_API uint64_t cb200_nvfp4_grouped_matmul_slice_m_workspace_size(const cb200_nvfp4_grouped_matmul_args *args);
+CB200_API int cb200_nvfp4_grouped_matmul_slice_m(const cb200_nvfp4_grouped_matmul_args *args, void *stream);
+
 /* ---- library / device state ---- */
 
 /* Reads and clears the status word kernels of this library write on the current device when a bounded

@@ -35,7 +35,9 @@ def refused(capi, name, args, **changes):
 
 def test_struct_layouts(capi):
     pairs = [("cb200_moe_route_args", capi.MoeRouteArgs), ("cb200_moe_dispatch_args", capi.MoeDispatchArgs),
-             ("cb200_moe_combine_args", capi.MoeCombineArgs), ("cb200_nvfp4_quantize_args", capi.Nvfp4QuantizeArgs)]
+             ("cb200_moe_combine_args", capi.MoeCombineArgs), ("cb200_nvfp4_quantize_args", capi.Nvfp4QuantizeArgs),
+             ("cb200_nvfp4_matmul_args", capi.Nvfp4MatmulArgs),
+             ("cb200_nvfp4_grouped_matmul_args", capi.Nvfp4GroupedMatmulArgs)]
     lines = []
     for cname, ctype in pairs:
         offsets = ", ".join(f"offsetof({cname}, {f[0]})" for f in ctype._fields_)
@@ -115,6 +117,30 @@ def test_nvfp4_quantize_refusals(capi):
     lib_bytes.argtypes = [ctypes.c_uint32, ctypes.c_uint32]
     for rows, k in ((0, 64), (1, 16), (128, 64), (129, 80), (1 << 20, 7168)):
         assert lib_bytes(rows, k) == capi.nvfp4_tiled_scale_bytes(rows, k)
+
+
+def test_nvfp4_matmul_refusals(capi):
+    dense = capi.Nvfp4MatmulArgs(m=16, n=64, k=64, d_type=1, a=256, b=256, scale_a=256, scale_b=256, d=256)
+    groups = capi.Nvfp4GroupedMatmulArgs(m=16, n=64, k=64, group_count=4, d_type=1, a=256, b=256, group_list=256, scale_a=256,
+                                         scale_b=256, d=256)
+    for name, ok in (("cb200_nvfp4_matmul", dense), ("cb200_nvfp4_grouped_matmul_slice_m", groups)):
+        assert accepted(capi, name, ok) == capi.SUCCESS
+        for change in (dict(k=0), dict(k=48), dict(d_type=3), dict(scale_b_layout=2), dict(flags=1), dict(a=None), dict(a=264),
+                       dict(b=None), dict(b=264), dict(scale_a=None), dict(scale_a=264), dict(scale_b=None), dict(d=None),
+                       dict(d=264), dict(d=257, n=65), dict(alpha=258), dict(m=1 << 31)):
+            assert refused(capi, name, ok, **change), (name, change)
+        assert not refused(capi, name, ok, m=0, a=None, d=None)
+        assert not refused(capi, name, ok, n=65, d=258)
+        assert capi._function(name, type(ok))(None, None) == capi.INVALID
+    assert refused(capi, "cb200_nvfp4_matmul", dense, scale_a_layout=2)
+    for change in (dict(group_count=0), dict(group_count=1025), dict(group_list=None), dict(group_list=260),
+                   dict(group_list_type=2), dict(group_list_kind=2)):
+        assert refused(capi, "cb200_nvfp4_grouped_matmul_slice_m", groups, **change), change
+    # only scales by rows, and row tables, need a workspace
+    assert capi.nvfp4_matmul_workspace_size(4096, 4096, 4096, 1, 1) == 0
+    assert capi.nvfp4_matmul_workspace_size(128, 256, 4096, 0, 1) == capi.nvfp4_tiled_scale_bytes(128, 4096)
+    assert capi.nvfp4_matmul_workspace_size(16, 256, 4096, 1, 0) == capi.nvfp4_tiled_scale_bytes(256, 4096)
+    assert capi.nvfp4_grouped_matmul_workspace_size(256, 4096, 7168, 64, 1) > 0
 
 
 def test_python_calls_check_their_tensors(capi):
