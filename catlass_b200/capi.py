@@ -520,47 +520,50 @@ def _function(name, args_t, result=ctypes.c_int):
     return fn
 
 
-def _buffer(t, nbytes, what, like=None):
-    """Address of a CUDA tensor used as a raw buffer of at least `nbytes` bytes; None stays None."""
+def _device(t, what):
+    """Index of the device of a CUDA tensor."""
+    if t is None or t.get_device() < 0:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _buffer(t, nbytes, what, device):
+    """Address of a tensor of that device used as a raw buffer of at least `nbytes` bytes; None stays None."""
     if t is None:
         return None
-    if not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous CUDA tensor")
+    if t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous tensor of device {device}")
     if t.nbytes < nbytes:
         raise ValueError(f"{what} holds {t.nbytes} bytes, {nbytes} are needed")
-    if like is not None and t.get_device() != like.get_device():
-        raise ValueError(f"{what} is on another device")
     return t.data_ptr()
 
 
-def _rows(t, rows, width, pitch, elem, what, like=None):
+def _rows(t, rows, width, pitch, elem, what, device):
     """As _buffer, for `rows` rows of `width` elements with `pitch` elements between them (a view with strided rows is
     taken: only the storage behind its first element has to be long enough)."""
+    if not pitch:
+        return _buffer(t, rows * width * elem, what, device)
     if t is None:
         return None
-    if not t.is_cuda:
-        raise ValueError(f"{what} must be a CUDA tensor")
-    need = ((rows - 1) * (pitch or width) + width) * elem if rows and width else 0
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be a tensor of device {device}")
+    need = ((rows - 1) * pitch + width) * elem if rows and width else 0
     have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
     if have < need:
         raise ValueError(f"{what} holds {have} bytes, {need} are needed")
-    if like is not None and t.get_device() != like.get_device():
-        raise ValueError(f"{what} is on another device")
     return t.data_ptr()
 
 
-def _enqueue(name, args, like, stream):
-    """Calls the library on the device of `like`, on `stream` or that device's current stream."""
+def _enqueue(name, args, device, stream):
+    """Calls the library on that device, on `stream` or the device's current stream."""
     import torch
-    fn = _function(name, type(args))
-    device = like.get_device()
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
+    fn = _prepared.get(name) or _function(name, type(args))
+    handle = torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
     if torch.cuda.current_device() == device:
-        _check(name, fn(ctypes.byref(args), stream.cuda_stream))
+        _check(name, fn(ctypes.byref(args), handle))
     else:
         with torch.cuda.device(device):
-            _check(name, fn(ctypes.byref(args), stream.cuda_stream))
+            _check(name, fn(ctypes.byref(args), handle))
 
 
 def _float_bytes(type_code, what):
@@ -574,13 +577,15 @@ def moe_route(logits, weights, ids, tokens, experts, top_k, score=ROUTE_SOFTMAX,
               token_count=None, stream=None):
     """logits [tokens][experts] -> weights fp32 and ids int32 [tokens][top_k], the experts with the largest scores (plus
     bias) of the best groups, ties to the lower index; id -1 and weight 0 where no expert is left."""
+    dev = _device(logits, "logits")
     out = tokens * top_k * 4
     args = MoeRouteArgs(tokens, experts, top_k, score, groups, groups if groups_kept is None else groups_kept,
                         group_score, ROUTE_RENORMALIZE if renormalize else 0, logits_type, scaling, logits_pitch,
-                        _rows(logits, tokens, experts, logits_pitch, _float_bytes(logits_type, "logits_type"), "logits"),
-                        _buffer(bias, experts * 4, "bias", logits), _buffer(token_count, 4, "token_count", logits),
-                        _buffer(weights, out, "weights", logits), _buffer(ids, out, "ids", logits))
-    _enqueue("cb200_moe_route", args, logits, stream)
+                        _rows(logits, tokens, experts, logits_pitch, _float_bytes(logits_type, "logits_type"), "logits",
+                              dev),
+                        _buffer(bias, experts * 4, "bias", dev), _buffer(token_count, 4, "token_count", dev),
+                        _buffer(weights, out, "weights", dev), _buffer(ids, out, "ids", dev))
+    _enqueue("cb200_moe_route", args, dev, stream)
 
 
 def moe_dispatch_workspace_size(tokens, experts, top_k):
@@ -609,35 +614,37 @@ def moe_dispatch(x, ids, weights, group_list, position, tokens, experts, top_k, 
     """ids, weights [tokens][top_k] of a router -> rows sorted by expert: group_list [experts], position [tokens][top_k]
     (row of each pair, -1 when dropped), row_index / row_weight [tokens * top_k], and x [tokens][k] written to its rows
     of q / scale in the format `fmt`.  workspace: moe_dispatch_workspace_size bytes."""
+    dev = _device(ids, "ids")
     rows = tokens * top_k
     x_bytes = _float_bytes(x_type, "x_type")
     q_bytes, scale_bytes = _dispatch_sizes(rows, k, fmt, x_bytes)
     index_bytes = 8 if row_index_type == GROUP_LIST_INT64 else 4
     args = MoeDispatchArgs(
         tokens, experts, top_k, k, fmt, x_type, expert_begin, group_list_type, group_list_kind, row_index_type, x_pitch,
-        None if fmt == DISPATCH_INDEX else _rows(x, tokens, k, x_pitch, x_bytes, "x", ids),
-        _buffer(ids, rows * 4, "ids"), _buffer(weights, rows * 4, "weights", ids),
-        _buffer(tensor_scale, 4, "tensor_scale", ids), _buffer(q, q_bytes, "q", ids),
-        _buffer(scale, scale_bytes, "scale", ids),
-        _buffer(group_list, experts * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", ids),
-        _buffer(position, rows * 4, "position", ids), _buffer(row_index, rows * index_bytes, "row_index", ids),
-        _buffer(row_weight, rows * 4, "row_weight", ids), _buffer(workspace, 0, "workspace", ids),
+        None if fmt == DISPATCH_INDEX else _rows(x, tokens, k, x_pitch, x_bytes, "x", dev),
+        _buffer(ids, rows * 4, "ids", dev), _buffer(weights, rows * 4, "weights", dev),
+        _buffer(tensor_scale, 4, "tensor_scale", dev), _buffer(q, q_bytes, "q", dev),
+        _buffer(scale, scale_bytes, "scale", dev),
+        _buffer(group_list, experts * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", dev),
+        _buffer(position, rows * 4, "position", dev), _buffer(row_index, rows * index_bytes, "row_index", dev),
+        _buffer(row_weight, rows * 4, "row_weight", dev), _buffer(workspace, 0, "workspace", dev),
         0 if workspace is None else workspace.nbytes)
-    _enqueue("cb200_moe_dispatch", args, ids, stream)
+    _enqueue("cb200_moe_dispatch", args, dev, stream)
 
 
 def moe_combine(d, position, weights, out, tokens, n, top_k, rows=None, d_type=DTYPE_BF16, out_type=DTYPE_BF16,
                 shared=None, shared_weight=1.0, stream=None):
     """out[t] = shared_weight * shared[t] + sum_j weights[t][j] * d[position[t][j]], d [rows][n] (rows: tokens * top_k
     unless given), slots with a negative position skipped."""
+    dev = _device(d, "d")
     rows = tokens * top_k if rows is None else rows
     out_bytes = tokens * n * _float_bytes(out_type, "out_type")
     args = MoeCombineArgs(tokens, top_k, n, rows, d_type, out_type, shared_weight, 0,
-                          _buffer(d, rows * n * _float_bytes(d_type, "d_type"), "d"),
-                          _buffer(position, tokens * top_k * 4, "position", d),
-                          _buffer(weights, tokens * top_k * 4, "weights", d), _buffer(shared, out_bytes, "shared", d),
-                          _buffer(out, out_bytes, "out", d))
-    _enqueue("cb200_moe_combine", args, d, stream)
+                          _buffer(d, rows * n * _float_bytes(d_type, "d_type"), "d", dev),
+                          _buffer(position, tokens * top_k * 4, "position", dev),
+                          _buffer(weights, tokens * top_k * 4, "weights", dev), _buffer(shared, out_bytes, "shared", dev),
+                          _buffer(out, out_bytes, "out", dev))
+    _enqueue("cb200_moe_combine", args, dev, stream)
 
 
 def nvfp4_tiled_scale_bytes(rows, k):
@@ -649,15 +656,16 @@ def nvfp4_quantize(x, q, scale, rows, k, tensor_scale, x_type=DTYPE_BF16, x_pitc
                    swiglu=False, row_count=None, row_count_type=GROUP_LIST_INT64, stream=None):
     """x [rows][k] (with swiglu [rows][2k]: act next to gate) -> q [rows][k/2] bytes and E4M3 scales by rows ([rows][k/16]
     bytes) or tiled (nvfp4_tiled_scale_bytes bytes), in units of the device scalar tensor_scale."""
+    dev = _device(x, "x")
     width = 2 * k if swiglu else k
     scale_bytes = nvfp4_tiled_scale_bytes(rows, k) if scale_layout == NVFP4_SCALES_TILED else rows * (k // 16)
     args = Nvfp4QuantizeArgs(
         rows, k, x_type, scale_layout, NVFP4_SWIGLU if swiglu else 0, row_count_type, x_pitch,
-        _rows(x, rows, width, x_pitch, _float_bytes(x_type, "x_type"), "x"),
-        _buffer(tensor_scale, 4, "tensor_scale", x),
-        _buffer(row_count, 8 if row_count_type == GROUP_LIST_INT64 else 4, "row_count", x),
-        _buffer(q, rows * (k // 2), "q", x), _buffer(scale, scale_bytes, "scale", x))
-    _enqueue("cb200_nvfp4_quantize", args, x, stream)
+        _rows(x, rows, width, x_pitch, _float_bytes(x_type, "x_type"), "x", dev),
+        _buffer(tensor_scale, 4, "tensor_scale", dev),
+        _buffer(row_count, 8 if row_count_type == GROUP_LIST_INT64 else 4, "row_count", dev),
+        _buffer(q, rows * (k // 2), "q", dev), _buffer(scale, scale_bytes, "scale", dev))
+    _enqueue("cb200_nvfp4_quantize", args, dev, stream)
 
 
 def _nvfp4_scale_bytes(rows, k, layout):
@@ -674,13 +682,14 @@ def nvfp4_matmul(a, b, scale_a, scale_b, d, m, n, k, workspace=None, alpha=None,
                  scale_b_layout=NVFP4_SCALES_ROWS, d_type=DTYPE_BF16, stream=None, block_num=0):
     """a [m][k/2], b [n][k/2] packed E2M1 with E4M3 scales by rows or tiled -> d [m][n] = alpha * a @ b^T.  alpha: device
     scalar (the product of the tensor scales); workspace: nvfp4_matmul_workspace_size bytes."""
+    dev = _device(a, "a")
     args = Nvfp4MatmulArgs(
-        m, n, k, scale_a_layout, scale_b_layout, d_type, _buffer(a, m * (k // 2), "a"), _buffer(b, n * (k // 2), "b", a),
-        _buffer(scale_a, _nvfp4_scale_bytes(m, k, scale_a_layout), "scale_a", a),
-        _buffer(scale_b, _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", a), _buffer(alpha, 4, "alpha", a),
-        _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", a), _buffer(workspace, 0, "workspace", a),
+        m, n, k, scale_a_layout, scale_b_layout, d_type, _buffer(a, m * (k // 2), "a", dev), _buffer(b, n * (k // 2), "b", dev),
+        _buffer(scale_a, _nvfp4_scale_bytes(m, k, scale_a_layout), "scale_a", dev),
+        _buffer(scale_b, _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", dev), _buffer(alpha, 4, "alpha", dev),
+        _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", dev), _buffer(workspace, 0, "workspace", dev),
         0 if workspace is None else workspace.nbytes, block_num, 0)
-    _enqueue("cb200_nvfp4_matmul", args, a, stream)
+    _enqueue("cb200_nvfp4_matmul", args, dev, stream)
 
 
 def nvfp4_grouped_matmul_workspace_size(m, n, k, group_count, scale_b_layout=NVFP4_SCALES_ROWS):
@@ -695,12 +704,13 @@ def nvfp4_grouped_matmul(a, b, group_list, scale_a, scale_b, d, m, n, k, group_c
                          group_list_kind=GROUP_LIST_SIZES, stream=None, block_num=0):
     """Grouped slice-M NVFP4 matmul: a [m][k/2], b [G][n][k/2], scale_a by rows, scale_b by rows or tiled per group,
     alpha [G] on the device; rows past the last group are not written."""
+    dev = _device(a, "a")
     args = Nvfp4GroupedMatmulArgs(
-        m, n, k, group_count, scale_b_layout, group_list_type, group_list_kind, d_type, _buffer(a, m * (k // 2), "a"),
-        _buffer(b, group_count * n * (k // 2), "b", a),
-        _buffer(group_list, group_count * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", a),
-        _buffer(scale_a, m * (k // 16), "scale_a", a),
-        _buffer(scale_b, group_count * _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", a),
-        _buffer(alpha, group_count * 4, "alpha", a), _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", a),
-        _buffer(workspace, 0, "workspace", a), 0 if workspace is None else workspace.nbytes, block_num, 0)
-    _enqueue("cb200_nvfp4_grouped_matmul_slice_m", args, a, stream)
+        m, n, k, group_count, scale_b_layout, group_list_type, group_list_kind, d_type, _buffer(a, m * (k // 2), "a", dev),
+        _buffer(b, group_count * n * (k // 2), "b", dev),
+        _buffer(group_list, group_count * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", dev),
+        _buffer(scale_a, m * (k // 16), "scale_a", dev),
+        _buffer(scale_b, group_count * _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", dev),
+        _buffer(alpha, group_count * 4, "alpha", dev), _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", dev),
+        _buffer(workspace, 0, "workspace", dev), 0 if workspace is None else workspace.nbytes, block_num, 0)
+    _enqueue("cb200_nvfp4_grouped_matmul_slice_m", args, dev, stream)
