@@ -34,6 +34,10 @@ struct NvPlan {
 // rows of A on one: a row tile that is mostly padding, or too few tiles to fill the SMs, is cheaper on the latter.
 bool nv_use_few(const NvProblem& q)
 {
+    const long v = dev_knob("CB200_NV_FEW", -1);
+    if (v >= 0) {
+        return v != 0;
+    }
     if (q.group_count != 0) {
         return q.m / q.group_count <= 64u;
     }
@@ -115,10 +119,19 @@ int encode_nv_rows(CUtensorMap* map, const NvProblem& q, uint32_t box_rows)
     return encode_tmap_u8(map, q.a, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int launch_nv_pair(const NvProblem& q, const NvPlan& plan, const NvParams& p, const DeviceState& dev,
-                   cudaStream_t stream)
+// D as bytes, boxes of 32 rows x 64 bytes.
+int encode_nv_output(CUtensorMap* map, const NvProblem& q)
 {
-    CUtensorMap tmap_a, tmap_b, tmap_sfa, tmap_sfb;
+    const uint64_t row_bytes = q.n * float_bytes(q.d_type);
+    const uint64_t dims[2] = {row_bytes, q.m};
+    const uint64_t strides[1] = {row_bytes};
+    const uint32_t box[2] = {64, 32};
+    return encode_tmap_u8(map, q.d, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+int launch_nv_pair(const NvProblem& q, const NvPlan& plan, NvParams p, const DeviceState& dev, cudaStream_t stream)
+{
+    CUtensorMap tmap_a, tmap_b, tmap_sfa, tmap_sfb, tmap_d;
     int rc = encode_nv_rows(&tmap_a, q, kBlockM);
     rc = rc != CB200_SUCCESS ? rc : encode_nv_weights(&tmap_b, q, plan);
     rc = rc != CB200_SUCCESS
@@ -128,6 +141,9 @@ int launch_nv_pair(const NvProblem& q, const NvPlan& plan, const NvParams& p, co
     rc = rc != CB200_SUCCESS
              ? rc
              : encode_nv_scales(&tmap_sfb, p.sfb, plan.words, static_cast<uint64_t>(plan.sfb_blocks) * plan.matrices);
+    p.tma_store = (q.n * float_bytes(q.d_type)) % 16u == 0 ? 1u : 0u;
+    tmap_d = tmap_a;  // (not read without tma_store)
+    rc = rc != CB200_SUCCESS || !p.tma_store ? rc : encode_nv_output(&tmap_d, q);
     if (rc != CB200_SUCCESS) {
         return rc;
     }
@@ -152,7 +168,7 @@ int launch_nv_pair(const NvProblem& q, const NvPlan& plan, const NvParams& p, co
     const uint64_t tiles = static_cast<uint64_t>(plan.max_tiles) * ((q.n + 255u) / 256u);
     pairs = tiles < pairs ? static_cast<uint32_t>(tiles) : pairs;
     CB200_CUDA_TRY(launch_dependent(nvfp4_pair_kernel, 2 * pairs, kNvPairThreads, NvPairSmem::kTotalBytes, stream,
-                                    tmap_a, tmap_b, tmap_sfa, tmap_sfb, p));
+                                    tmap_a, tmap_b, tmap_sfa, tmap_sfb, tmap_d, p));
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return CB200_SUCCESS;
 }
@@ -298,6 +314,7 @@ int run_nv(const NvProblem& q, void* stream_v)
     p.status = dev->status;
     p.table = q.group_count != 0 ? table : nullptr;
     p.num_row_tiles = q.group_count != 0 ? num_tiles : nullptr;
+    p.tma_store = 0;
     return plan.few ? launch_nv_few(q, plan, p, *dev, stream) : launch_nv_pair(q, plan, p, *dev, stream);
 }
 

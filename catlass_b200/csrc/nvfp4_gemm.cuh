@@ -34,6 +34,7 @@ struct NvParams {
     unsigned* status;
     const int4* table;             // grouped: [row tile] = (first row, one past the group's last row, group, 0)
     const uint32_t* num_row_tiles; // grouped: entries of the table
+    uint32_t tma_store;            // pair kernel: D has a tensor map
 };
 
 // Instruction descriptor of kind::mxf4nvf4 with E4M3 scales (bit 23 = 0); with 16-element blocks an MMA uses all four
@@ -236,14 +237,18 @@ struct NvPairSmem {
     static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
     static constexpr int kRingBytes = kNvPairStages * kStageBytes;
     static constexpr int kBarriers = 3 * kNvPairStages + 2;
-    // rows of D that do not start on 16-byte boundaries leave through a slab per epilogue warp: 32 rows x 32 two-byte or
-    // 16 four-byte columns, 17 words apart (an odd number: rows fall on different banks)
-    static constexpr int kSlabBytes = 32 * 17 * 4;
-    static constexpr int kSlabOffset = kRingBytes + kBarriers * 8 + 16;
-    static constexpr int kTotalBytes = 1024 + kSlabOffset + kNvPairEpiWarps * kSlabBytes;
+    // D leaves through a slab per epilogue warp: 32 rows x 64 bytes for a TMA store (64-byte swizzle, so slabs start on
+    // 512-byte boundaries), or, where D's rows do not start on 16-byte boundaries, 32 rows 17 words apart (an odd
+    // number: rows fall on different banks)
+    static constexpr int kSlabBytes = 2048;
+    static constexpr int kOddSlabBytes = 32 * 17 * 4;
+    static constexpr int kSlabOffset = kRingBytes;
+    static constexpr int kBarrierOffset = kSlabOffset + kNvPairEpiWarps * kOddSlabBytes;
+    static constexpr int kTotalBytes = 1024 + kBarrierOffset + kBarriers * 8 + 16;
 };
 static_assert(NvPairSmem::kTotalBytes <= 227 * 1024, "shared memory budget");
 static_assert(NvPairSmem::kStageBytes % 1024 == 0, "swizzled tiles start on 1 KB boundaries");
+static_assert(NvPairSmem::kBarrierOffset % 8 == 0 && NvPairSmem::kSlabBytes <= NvPairSmem::kOddSlabBytes, "slabs");
 
 // One row's `kCount` accumulator columns (fp32 bit patterns) starting at col, times alpha, to D.
 template <int kCount>
@@ -339,12 +344,53 @@ __device__ __forceinline__ void nv_store_rows_staged(const NvParams& p, const ui
     }
 }
 
+// A warp's 32 rows x 64 bytes of D (kCount columns from r, times alpha) by one TMA store.  Every store instruction of the
+// row-per-lane form above touches 32 rows, 16 bytes each; 256 x 256 tiles took 1.8 us longer that way, and the last one 3.6.
+// The slab's previous store has been read (the caller waits).  All lanes take part; the rows are all to be stored.
+template <int kCount>
+__device__ __forceinline__ void nv_tma_store(const NvParams& p, const CUtensorMap* tmap_d, const uint32_t* r, uint8_t* slab,
+                                             uint32_t row0, uint32_t col, float alpha, uint32_t lane)
+{
+    uint8_t* row = slab + lane * 64;
+    const uint32_t swizzle = (lane >> 1) & 3u;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kCount == 16) {
+                w[i] = __float_as_uint(__uint_as_float(r[4 * c + i]) * alpha);
+            } else {
+                w[i] = pack_out2(__uint_as_float(r[8 * c + 2 * i]) * alpha, __uint_as_float(r[8 * c + 2 * i + 1]) * alpha,
+                                 p.d_type == 2);
+            }
+        }
+        *reinterpret_cast<uint4*>(row + ((c ^ swizzle) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(tmap_d, smem_u32(slab), static_cast<int32_t>(col * (64 / kCount)), static_cast<int32_t>(row0));
+        tma_store_commit();
+    }
+}
+
+// The lane that issues a warp's stores waits until they have read the slab; then the warp may write it again.
+__device__ __forceinline__ void nv_slab_free(uint32_t lane)
+{
+    if (lane == 0) {
+        tma_store_wait_read<0>();
+    }
+    __syncwarp();
+}
+
 // tmap_b: {row bytes, n, groups}, boxes of 128 rows; tmap_sfa / tmap_sfb: the tiled scales as {256, 2 * words, row
-// blocks}, boxes of {256, 8, 1} = four words; words past the last read as zero.
+// blocks}, boxes of {256, 8, 1} = four words; words past the last read as zero; tmap_d: D as bytes, boxes of
+// 64 bytes x 32 rows (p.tma_store).
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
 nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                   const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
-                  const NvParams p)
+                  const __grid_constant__ CUtensorMap tmap_d, const NvParams p)
 {
     using S = NvPairSmem;
     constexpr int kStages = kNvPairStages;
@@ -358,7 +404,7 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
     uint8_t* smem = smem_raw + pad;
     const uint32_t ring = raw_addr + pad;
-    uint64_t* s_bars = reinterpret_cast<uint64_t*>(smem + S::kRingBytes);
+    uint64_t* s_bars = reinterpret_cast<uint64_t*>(smem + S::kBarrierOffset);
     const uint32_t bar_full = smem_u32(s_bars);               // leader: operands and scales of both CTAs landed
     const uint32_t bar_empty = bar_full + kStages * 8;        // both: the stage's MMAs completed
     const uint32_t bar_sf_full = bar_empty + kStages * 8;     // leader: scales copied into both TMEMs
@@ -562,8 +608,8 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         const uint32_t quad = warp & 3;                           // TMEM lane quarter this warp may read
         const uint32_t part = (warp - 3 - kNvPairCopiers) >> 2;   // which 64 columns of the tile's 256
         const bool staged = (p.n & (p.d_type == 0 ? 3u : 7u)) != 0;
-        uint32_t* slab = reinterpret_cast<uint32_t*>(smem + S::kSlabOffset) +
-                         (warp - 3 - kNvPairCopiers) * (S::kSlabBytes / 4);
+        uint8_t* slab = smem + S::kSlabOffset +
+                        (warp - 3 - kNvPairCopiers) * (staged ? S::kOddSlabBytes : S::kSlabBytes);
         uint32_t acc_phase = 0;
         bool ok = true;
         for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
@@ -591,19 +637,40 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             acc_phase ^= 1;
             const uint32_t row0 = static_cast<uint32_t>(tile_row0) + cta_rank * kBlockM + quad * 32, row = row0 + lane;
             const uint32_t col = nt * kMxBlockN + part * 64;
+            if (col >= p.n || row0 >= static_cast<uint32_t>(row_end)) {
+                continue;
+            }
             if (staged) {
-                if (col < p.n) {
-                    nv_store_rows_staged(p, r[0], slab, row0, static_cast<uint32_t>(row_end), col, alpha, lane);
-                }
+                uint32_t* words = reinterpret_cast<uint32_t*>(slab);
+                nv_store_rows_staged(p, r[0], words, row0, static_cast<uint32_t>(row_end), col, alpha, lane);
                 if (col + 32 < p.n) {
-                    nv_store_rows_staged(p, r[1], slab, row0, static_cast<uint32_t>(row_end), col + 32, alpha, lane);
+                    nv_store_rows_staged(p, r[1], words, row0, static_cast<uint32_t>(row_end), col + 32, alpha, lane);
                 }
-            } else if (static_cast<int32_t>(row) < row_end && col < p.n) {
+            } else if (p.tma_store && row0 + 32 <= static_cast<uint32_t>(row_end)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (p.d_type == 0) {
+#pragma unroll
+                        for (int f = 0; f < 2; ++f) {
+                            if (col + h * 32 + f * 16 < p.n) {
+                                nv_slab_free(lane);
+                                nv_tma_store<16>(p, &tmap_d, r[h] + f * 16, slab, row0, col + h * 32 + f * 16, alpha, lane);
+                            }
+                        }
+                    } else if (col + h * 32 < p.n) {
+                        nv_slab_free(lane);
+                        nv_tma_store<32>(p, &tmap_d, r[h], slab, row0, col + h * 32, alpha, lane);
+                    }
+                }
+            } else if (row < static_cast<uint32_t>(row_end)) {
                 nv_store_row<32>(p, r[0], row, col, alpha);
                 if (col + 32 < p.n) {
                     nv_store_row<32>(p, r[1], row, col + 32, alpha);
                 }
             }
+        }
+        if (lane == 0) {
+            tma_store_wait_all<0>();
         }
     }
 
