@@ -447,6 +447,10 @@ int cb200_nvfp4_quantize(const cb200_nvfp4_quantize_args* a, void* stream_v)
     const uint64_t want = (static_cast<uint64_t>(p.rows) * p.blocks + kNvQuantThreads - 1) / kNvQuantThreads;
     const uint64_t cap = static_cast<uint64_t>(dev->sm_count) * 8u;
     const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
+    p.word_stores = p.blocks % 4u == 0 && aligned_to(a->scale, 4) ? 1u : 0u;
+    p.step_rows = grid * kNvQuantThreads / p.blocks;
+    p.step_blocks = grid * kNvQuantThreads % p.blocks;
+    p.step_elements = p.step_rows * p.pitch + static_cast<uint64_t>(p.step_blocks) * 16u;
     if (swiglu) {
         launch_nv_quant<true>(p, a->x_type, grid, stream);
     } else {

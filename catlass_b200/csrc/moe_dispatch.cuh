@@ -385,7 +385,7 @@ moe_rows_kernel(const DispatchParams p)
             block_max = fmaxf(block_max, __shfl_xor_sync(0xffffffffu, block_max, 1));
             codes = mx_e4m3_codes16<kType>(v, block_max, scale_byte);
         } else {
-            const uint2 packed = nvfp4_block(v, tensor_scale, scale_byte);
+            const uint2 packed = nvfp4_block(v, amax_bits16(v), tensor_scale, scale_byte);
             codes.x = packed.x;
             codes.y = packed.y;
         }

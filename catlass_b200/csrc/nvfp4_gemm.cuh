@@ -6,7 +6,7 @@
 //
 //   nvfp4_pack_scales_kernel  scales by rows -> tiled; for a grouped problem also the row-tile table: tiles start at a
 //                             group's first row, so their scale blocks do too.
-//   nvfp4_pair_kernel         CTA pairs (cta_group::2), tile 256 x 256: prompts.  Tensor-bound.
+//   nvfp4_pair_kernel         CTA pairs (cta_group::2): 256 weight rows on the M axis, up to 256 rows of A on the N axis.
 //   nvfp4_few_kernel          (nvfp4_few.cuh) weights on the M axis, up to 128 rows of A on the N axis: HBM-bound.
 #pragma once
 
@@ -222,180 +222,119 @@ nvfp4_pack_scales_kernel(const NvPackParams p)
     }
 }
 
-// ---------------------------------------------------------------- CTA pairs, 256 x 256 tiles
-
+// ---------------------------------------------------------------- CTA pairs
+//
+// The problem lies transposed on the tensor core: a tile is 256 WEIGHT rows (the M axis; CTA r of the pair owns rows
+// [128 r, 128 r + 128) and their accumulator lanes) and up to 256 rows of A (the N axis, in steps of 32).  A group's last
+// rows then cost what they are: an MMA of N columns takes N/256 of a full one and reads N/256 of A, where rows of A on the
+// M axis would be padded to 256.  And a warp that stores a row of D writes 32 neighbouring columns.
+//
+// Per stage (256 along K) a CTA takes in its weights 16 KB, half of the tile's rows of A (up to 16 KB) and the scale blocks
+// of its weight rows (2 KB) and of all rows of A (2 x 2 KB), and the tensor core reads 16 + 16 + 6 KB of it: 76 KB through
+// a shared memory of 128 bytes a clock are 608 clocks, against 512 of MMAs.  Measured with a full tile: 714 a stage.
 constexpr int kNvPairStages = 5;
 constexpr int kNvPairCopiers = 4;
 constexpr int kNvPairEpiWarps = 16;
+constexpr uint32_t kNvTileW = 256;  // weight rows per tile
+constexpr uint32_t kNvTileX = 256;  // rows of A per tile
 // warps: 0 operand producer, 1 MMA issuer, 2 scale producer, 3-6 scale copiers, 7-22 epilogue
 constexpr int kNvPairThreads = (3 + kNvPairCopiers + kNvPairEpiWarps) * 32;
 
 struct NvPairSmem {
-    static constexpr int kABytes = kBlockM * kBlockKBytes;          // 16 KB: this CTA's 128 rows of A
-    static constexpr int kBBytes = (kMxBlockN / 2) * kBlockKBytes;  // 16 KB: this CTA's half of B
-    static constexpr int kSfBytes = 3 * 2048;                       // four words each of A, B block 0, B block 1
-    static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
+    static constexpr int kWBytes = 128 * kBlockKBytes;   // this CTA's 128 weight rows
+    static constexpr int kXBytes = 128 * kBlockKBytes;   // its half of the rows of A
+    static constexpr int kSfBytes = 3 * 2048;            // four words each of the weights and of A's two blocks
+    static constexpr int kStageBytes = kWBytes + kXBytes + kSfBytes;
     static constexpr int kRingBytes = kNvPairStages * kStageBytes;
-    static constexpr int kBarriers = 3 * kNvPairStages + 2;
-    // D leaves through a slab per epilogue warp: 32 rows x 64 bytes for a TMA store (64-byte swizzle, so slabs start on
-    // 512-byte boundaries), or, where D's rows do not start on 16-byte boundaries, 32 rows 17 words apart (an odd
-    // number: rows fall on different banks)
+    // 32 rows of D x 64 bytes (fp32: 16 x 128) per epilogue warp, on their way out by TMA stores
     static constexpr int kSlabBytes = 2048;
-    static constexpr int kOddSlabBytes = 32 * 17 * 4;
-    static constexpr int kSlabOffset = kRingBytes;
-    static constexpr int kBarrierOffset = kSlabOffset + kNvPairEpiWarps * kOddSlabBytes;
+    static constexpr int kBarrierOffset = kRingBytes + kNvPairEpiWarps * kSlabBytes;
+    static constexpr int kBarriers = 3 * kNvPairStages + 2;
     static constexpr int kTotalBytes = 1024 + kBarrierOffset + kBarriers * 8 + 16;
 };
 static_assert(NvPairSmem::kTotalBytes <= 227 * 1024, "shared memory budget");
 static_assert(NvPairSmem::kStageBytes % 1024 == 0, "swizzled tiles start on 1 KB boundaries");
-static_assert(NvPairSmem::kBarrierOffset % 8 == 0 && NvPairSmem::kSlabBytes <= NvPairSmem::kOddSlabBytes, "slabs");
 
-// One row's `kCount` accumulator columns (fp32 bit patterns) starting at col, times alpha, to D.
+// One warp's share of an accumulator whose lanes are columns of D: 32 columns (lane = column) of rows row0 .. row0 + rows,
+// r[i] being row i.  Every store instruction writes 32 neighbouring columns.
 template <int kCount>
-__device__ __forceinline__ void nv_store_row(const NvParams& p, const uint32_t (&r)[kCount], uint32_t row, uint32_t col,
-                                             float alpha)
+__device__ __forceinline__ void nv_store_columns(const NvParams& p, const uint32_t (&r)[kCount], uint32_t row0,
+                                                 uint32_t rows, uint32_t col, float alpha)
 {
-    const uint64_t at = static_cast<uint64_t>(row) * p.n + col;
-    const bool whole = col + kCount <= p.n;
+    const uint64_t at = static_cast<uint64_t>(row0) * p.n + col;
+    if (col >= p.n) {
+        return;
+    }
     if (p.d_type == 0) {
         float* d = static_cast<float*>(p.d) + at;
-        if (whole && (p.n & 3u) == 0) {
 #pragma unroll
-            for (int v = 0; v < kCount / 4; ++v) {
-                reinterpret_cast<float4*>(d)[v] =
-                    make_float4(__uint_as_float(r[4 * v]) * alpha, __uint_as_float(r[4 * v + 1]) * alpha,
-                                __uint_as_float(r[4 * v + 2]) * alpha, __uint_as_float(r[4 * v + 3]) * alpha);
+        for (int i = 0; i < kCount; ++i) {
+            if (static_cast<uint32_t>(i) < rows) {
+                *d = __uint_as_float(r[i]) * alpha;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kCount; ++i) {
-                if (col + i < p.n) {
-                    d[i] = __uint_as_float(r[i]) * alpha;
-                }
-            }
-        }
-        return;
-    }
-    const bool f16 = p.d_type == 2;
-    uint16_t* d = static_cast<uint16_t*>(p.d) + at;
-    uint32_t packed[kCount / 2];
-#pragma unroll
-    for (int i = 0; i < kCount / 2; ++i) {
-        packed[i] = pack_out2(__uint_as_float(r[2 * i]) * alpha, __uint_as_float(r[2 * i + 1]) * alpha, f16);
-    }
-    if (whole && (p.n & 7u) == 0) {
-#pragma unroll
-        for (int v = 0; v < kCount / 8; ++v) {
-            reinterpret_cast<uint4*>(d)[v] =
-                make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
+            d += p.n;
         }
     } else {
+        uint16_t* d = static_cast<uint16_t*>(p.d) + at;
+        const bool f16 = p.d_type == 2;
 #pragma unroll
-        for (int i = 0; i < kCount / 2; ++i) {
-            if (col + 2 * i < p.n) {
-                d[2 * i] = static_cast<uint16_t>(packed[i]);
+        for (int i = 0; i < kCount; ++i) {
+            if (static_cast<uint32_t>(i) < rows) {
+                *d = pack_out1(__uint_as_float(r[i]) * alpha, f16);
             }
-            if (col + 2 * i + 1 < p.n) {
-                d[2 * i + 1] = static_cast<uint16_t>(packed[i] >> 16);
-            }
+            d += p.n;
         }
     }
 }
 
-// The same for a whole warp (lane = row, rows row0 + lane < row_end), every store instruction covering 32 consecutive
-// columns of one row: for rows of D that start anywhere.  One row per lane there means 32 two-byte pieces of 32 rows per
-// instruction (4111 x 515 x 7168: 61 us, against 24 us this way).  All lanes take part.
-__device__ __forceinline__ void nv_store_rows_staged(const NvParams& p, const uint32_t (&r)[32], uint32_t* slab,
-                                                     uint32_t row0, uint32_t row_end, uint32_t col, float alpha,
-                                                     uint32_t lane)
-{
-    const uint32_t rows = row0 >= row_end ? 0u : (row_end - row0 < 32u ? row_end - row0 : 32u);
-    if (p.d_type == 0) {
-        for (uint32_t h = 0; h < 2; ++h) {
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                slab[lane * 17 + i] = __float_as_uint(__uint_as_float(h == 0 ? r[i] : r[16 + i]) * alpha);
-            }
-            __syncwarp();
-            const uint32_t c = col + h * 16 + (lane & 15u);  // two rows per step
-            for (uint32_t q = lane >> 4; q < rows; q += 2) {
-                if (c < p.n) {
-                    static_cast<uint32_t*>(p.d)[static_cast<uint64_t>(row0 + q) * p.n + c] = slab[q * 17 + (lane & 15u)];
-                }
-            }
-        }
-        return;
-    }
-    const bool f16 = p.d_type == 2;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        slab[lane * 17 + i] = pack_out2(__uint_as_float(r[2 * i]) * alpha, __uint_as_float(r[2 * i + 1]) * alpha, f16);
-    }
-    __syncwarp();
-    const uint16_t* half = reinterpret_cast<const uint16_t*>(slab) + lane;
-    if (col + lane < p.n) {
-        uint16_t* d = static_cast<uint16_t*>(p.d) + static_cast<uint64_t>(row0) * p.n + col + lane;
-#pragma unroll 8
-        for (uint32_t q = 0; q < rows; ++q) {
-            d[static_cast<uint64_t>(q) * p.n] = half[q * 34];
-        }
-    }
-}
-
-// A warp's 32 rows x 64 bytes of D (kCount columns from r, times alpha) by one TMA store.  Every store instruction of the
-// row-per-lane form above touches 32 rows, 16 bytes each; 256 x 256 tiles took 1.8 us longer that way, and the last one 3.6.
-// The slab's previous store has been read (the caller waits).  All lanes take part; the rows are all to be stored.
+// The same 32 columns of kCount whole rows through a slab and one TMA store (every thread writes its column, two bytes at a
+// time: 32 lanes, 64 neighbouring bytes).  The slab's previous store is waited for.  All lanes take part.
 template <int kCount>
-__device__ __forceinline__ void nv_tma_store(const NvParams& p, const CUtensorMap* tmap_d, const uint32_t* r, uint8_t* slab,
-                                             uint32_t row0, uint32_t col, float alpha, uint32_t lane)
-{
-    uint8_t* row = slab + lane * 64;
-    const uint32_t swizzle = (lane >> 1) & 3u;
-#pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (kCount == 16) {
-                w[i] = __float_as_uint(__uint_as_float(r[4 * c + i]) * alpha);
-            } else {
-                w[i] = pack_out2(__uint_as_float(r[8 * c + 2 * i]) * alpha, __uint_as_float(r[8 * c + 2 * i + 1]) * alpha,
-                                 p.d_type == 2);
-            }
-        }
-        *reinterpret_cast<uint4*>(row + ((c ^ swizzle) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_2d(tmap_d, smem_u32(slab), static_cast<int32_t>(col * (64 / kCount)), static_cast<int32_t>(row0));
-        tma_store_commit();
-    }
-}
-
-// The lane that issues a warp's stores waits until they have read the slab; then the warp may write it again.
-__device__ __forceinline__ void nv_slab_free(uint32_t lane)
+__device__ __forceinline__ void nv_tma_store_columns(const NvParams& p, const CUtensorMap* tmap_d, const uint32_t* r,
+                                                     uint8_t* slab, uint32_t row0, uint32_t col0, float alpha,
+                                                     uint32_t lane)
 {
     if (lane == 0) {
         tma_store_wait_read<0>();
     }
     __syncwarp();
+    constexpr uint32_t kElem = 64 / kCount;  // 32 rows of two-byte, 16 of four-byte elements
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+        const float v = __uint_as_float(r[i]) * alpha;
+        if constexpr (kElem == 4) {
+            reinterpret_cast<float*>(slab)[i * 32 + lane] = v;
+        } else {
+            reinterpret_cast<uint16_t*>(slab)[i * 32 + lane] = pack_out1(v, p.d_type == 2);
+        }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(tmap_d, smem_u32(slab), static_cast<int32_t>(col0 * kElem), static_cast<int32_t>(row0));
+        tma_store_commit();
+    }
 }
 
-// tmap_b: {row bytes, n, groups}, boxes of 128 rows; tmap_sfa / tmap_sfb: the tiled scales as {256, 2 * words, row
-// blocks}, boxes of {256, 8, 1} = four words; words past the last read as zero; tmap_d: D as bytes, boxes of
-// 64 bytes x 32 rows (p.tma_store).
+// Rows of A as a tensor {row bytes, m}, boxes of 16, 32, 64 and 128 rows.  A tile's share of a CTA is one box, the smallest
+// that holds it: a TMA instruction costs its thread ~65 ns, and eight boxes of 16 rows a stage set the kernel's pace (0.59
+// us a stage instead of 0.38).
+struct NvRowMaps {
+    CUtensorMap box[4];
+};
+
+// tmap_w: {row bytes, n, groups}, boxes of 128 rows; tmap_sfw / tmap_sfx: the tiled scales as {256, 2 * words, row blocks},
+// boxes of {256, 8, 1} = four words; words past the last read as zero; tmap_d: D as bytes, boxes of 64 bytes x 32 rows, fp32
+// 128 x 16 (p.tma_store).
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvPairThreads, 1)
-nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                  const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
+nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ NvRowMaps tmap_x,
+                  const __grid_constant__ CUtensorMap tmap_sfw, const __grid_constant__ CUtensorMap tmap_sfx,
                   const __grid_constant__ CUtensorMap tmap_d, const NvParams p)
 {
     using S = NvPairSmem;
     constexpr int kStages = kNvPairStages;
-    constexpr uint32_t kAccCols = kMxBlockN;
-    constexpr uint32_t kSfSlot = 48;  // one scale slot: A 16 columns, B 32
+    constexpr uint32_t kAccCols = kNvTileX;
+    constexpr uint32_t kSfSlot = 48;  // one scale slot: weights 16 columns, rows of A 32
     constexpr uint32_t kTmemCols = 512;
     static_assert(kAccCols + kStages * kSfSlot <= kTmemCols, "TMEM budget");
 
@@ -430,10 +369,10 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         mbar_init(bar_tmem_full, 1);
         mbar_init(bar_tmem_empty, 2 * kNvPairEpiWarps);
         fence_mbar_init();
-        prefetch_tmap(&tmap_a);
-        prefetch_tmap(&tmap_b);
-        prefetch_tmap(&tmap_sfa);
-        prefetch_tmap(&tmap_sfb);
+        prefetch_tmap(&tmap_w);
+        prefetch_tmap(&tmap_x.box[3]);
+        prefetch_tmap(&tmap_sfw);
+        prefetch_tmap(&tmap_sfx);
     }
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(s_tmem_ptr), kTmemCols);
@@ -447,21 +386,34 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     grid_launch_dependents();
     grid_dependency_wait();  // the packed scales, the table and the operands of the kernels before
 
-    const uint32_t m_tiles = grouped ? *p.num_row_tiles : (p.m + 2 * kBlockM - 1) / (2 * kBlockM);
-    const uint32_t n_tiles = (p.n + kMxBlockN - 1) / kMxBlockN;
+    const uint32_t m_tiles = grouped ? *p.num_row_tiles : (p.m + kNvTileX - 1) / kNvTileX;
+    const uint32_t n_tiles = (p.n + kNvTileW - 1) / kNvTileW;
     const uint32_t total_tiles = m_tiles * n_tiles;
     const uint32_t num_kb = p.num_k_blocks;
-    auto row_tile = [&](uint32_t mt, int32_t& row0, int32_t& row_end, int32_t& group) {
+    struct Tile {
+        uint32_t mt, nt;    // row tile of A, weight tile
+        uint32_t row0;      // first row of A
+        uint32_t rows;      // rows of A to store, 1 .. 256
+        uint32_t cols;      // ... padded to a multiple of 32: columns of the MMA
+        uint32_t group;
+    };
+    auto get = [&](uint32_t idx) {
+        Tile t;
+        mx_tile_coords(idx, m_tiles, n_tiles, p.band_rows, t.mt, t.nt);
+        uint32_t end;
         if (grouped) {
-            const int4 e = __ldg(p.table + mt);
-            row0 = e.x;
-            row_end = e.y;
-            group = e.z;
+            const int4 e = __ldg(p.table + t.mt);
+            t.row0 = static_cast<uint32_t>(e.x);
+            end = static_cast<uint32_t>(e.y);
+            t.group = static_cast<uint32_t>(e.z);
         } else {
-            row0 = static_cast<int32_t>(mt) * 2 * kBlockM;
-            row_end = static_cast<int32_t>(p.m);
-            group = 0;
+            t.row0 = t.mt * kNvTileX;
+            end = p.m;
+            t.group = 0;
         }
+        t.rows = end - t.row0 < kNvTileX ? end - t.row0 : kNvTileX;
+        t.cols = (t.rows + 31u) & ~31u;
+        return t;
     };
 
     if (warp == 0) {
@@ -470,25 +422,27 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
-                uint32_t mt, nt;
-                mx_tile_coords(idx, m_tiles, n_tiles, p.band_rows, mt, nt);
-                int32_t tile_row0, row_end, group;
-                row_tile(mt, tile_row0, row_end, group);
-                const int32_t row0 = tile_row0 + static_cast<int32_t>(cta_rank * kBlockM);
-                const int32_t col0 = static_cast<int32_t>(nt * kMxBlockN + cta_rank * (kMxBlockN / 2));
+                const Tile t = get(idx);
+                const uint32_t half = t.cols / 2;                          // this CTA's rows of A: 16 .. 128
+                const uint32_t which = half <= 16 ? 0u : (half <= 32 ? 1u : (half <= 64 ? 2u : 3u));
+                const uint32_t x_bytes = (16u << which) * kBlockKBytes;
+                const uint32_t x0 = t.row0 + cta_rank * half;
+                const uint32_t w0 = t.nt * kNvTileW + cta_rank * 128;
+                const uint32_t sf_x = t.cols > 128 ? 4096u : 2048u;
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_empty + stage * 8, phase ^ 1, s_abort, p.status, kDevTimeoutProducer);
                     if (!ok) {
                         break;
                     }
-                    const uint32_t sa = ring + stage * S::kStageBytes;
+                    const uint32_t sw = ring + stage * S::kStageBytes;
+                    const uint32_t sx = sw + S::kWBytes;
                     const int32_t k0 = static_cast<int32_t>(kb) * kBlockKBytes;
                     if (cta_rank == 0) {  // both CTAs' tiles and scale blocks
-                        mbar_expect_tx(bar_full + stage * 8, 2 * S::kStageBytes);
+                        mbar_expect_tx(bar_full + stage * 8, 2 * (S::kWBytes + x_bytes + 2048 + sf_x));
                     }
                     const uint32_t full = map_to_cta(bar_full + stage * 8, 0);  // the leader's barrier
-                    tma_load_2d_pair(sa, &tmap_a, full, k0, row0);
-                    tma_load_3d_pair(sa + S::kABytes, &tmap_b, full, k0, col0, group);
+                    tma_load_3d_pair(sw, &tmap_w, full, k0, static_cast<int32_t>(w0), static_cast<int32_t>(t.group));
+                    tma_load_2d_pair(sx, &tmap_x.box[which], full, k0, static_cast<int32_t>(x0));
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
@@ -503,25 +457,24 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
-                uint32_t mt, nt;
-                mx_tile_coords(idx, m_tiles, n_tiles, p.band_rows, mt, nt);
-                int32_t tile_row0, row_end, group;
-                row_tile(mt, tile_row0, row_end, group);
-                const int32_t block_a = static_cast<int32_t>(2 * mt + cta_rank);
-                const int32_t block_b = group * static_cast<int32_t>(p.sfb_blocks) + static_cast<int32_t>(2 * nt);
+                const Tile t = get(idx);
+                const int32_t block_w = static_cast<int32_t>(t.group * p.sfb_blocks + 2 * t.nt + cta_rank);
+                const int32_t block_x = static_cast<int32_t>(2 * t.mt);
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_empty + stage * 8, phase ^ 1, s_abort, p.status, kDevTimeoutProducer);
                     if (!ok) {
                         break;
                     }
-                    const uint32_t ssf = ring + stage * S::kStageBytes + S::kABytes + S::kBBytes;
+                    const uint32_t ssf = ring + stage * S::kStageBytes + S::kWBytes + S::kXBytes;
                     const uint32_t full = map_to_cta(bar_full + stage * 8, 0);
                     const int32_t w2 = static_cast<int32_t>(kb * 8);  // rows of 256 bytes, two per word
-                    // (a block past the last, of A or of B, reads zeros or another group's scales: its rows and
-                    // columns are not stored)
-                    tma_load_3d_pair(ssf, &tmap_sfa, full, 0, w2, block_a);
-                    tma_load_3d_pair(ssf + 2048, &tmap_sfb, full, 0, w2, block_b);
-                    tma_load_3d_pair(ssf + 4096, &tmap_sfb, full, 0, w2, block_b + 1);
+                    // (a block past the last, of A or of the weights, reads zeros or another group's scales: its rows
+                    // and columns are not stored)
+                    tma_load_3d_pair(ssf, &tmap_sfw, full, 0, w2, block_w);
+                    tma_load_3d_pair(ssf + 2048, &tmap_sfx, full, 0, w2, block_x);
+                    if (t.cols > 128) {
+                        tma_load_3d_pair(ssf + 4096, &tmap_sfx, full, 0, w2, block_x + 1);
+                    }
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
@@ -533,10 +486,10 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (leader CTA only)
         if (lane == 0 && cta_rank == 0) {
-            constexpr uint32_t idesc = make_idesc_nv(2 * kBlockM, kMxBlockN);
             uint32_t stage = 0, phase = 0, acc_phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
+                const uint32_t idesc = make_idesc_nv(kNvTileW, get(idx).cols);
                 ok = mbar_wait(bar_tmem_empty, acc_phase ^ 1, s_abort, p.status, kDevTimeoutMmaTmem);
                 if (!ok) {
                     break;
@@ -549,15 +502,15 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t sa = ring + stage * S::kStageBytes;
-                    const uint32_t sb = sa + S::kABytes;
-                    const uint32_t t_sfa = tmem_base + kAccCols + stage * kSfSlot;
-                    const uint32_t t_sfb = t_sfa + 16;
+                    const uint32_t sw = ring + stage * S::kStageBytes;
+                    const uint32_t sx = sw + S::kWBytes;
+                    const uint32_t t_sfw = tmem_base + kAccCols + stage * kSfSlot;
+                    const uint32_t t_sfx = t_sfw + 16;
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
-                        const uint64_t da = make_smem_desc_sw128(sa + j * 32, 16, 1024);
-                        const uint64_t db = make_smem_desc_sw128(sb + j * 32, 16, 1024);
-                        umma_nv<2>(tmem_base, da, db, idesc, (kb | j) != 0 ? 1u : 0u, t_sfa + j * 4, t_sfb + j * 8);
+                        const uint64_t dw = make_smem_desc_sw128(sw + j * 32, 16, 1024);
+                        const uint64_t dx = make_smem_desc_sw128(sx + j * 32, 16, 1024);
+                        umma_nv<2>(tmem_base, dw, dx, idesc, (kb | j) != 0 ? 1u : 0u, t_sfw + j * 4, t_sfx + j * 8);
                     }
                     umma_commit_pair(bar_empty + stage * 8, 0x3);  // frees the stage and its TMEM slot in both CTAs
                     if (++stage == kStages) {
@@ -575,25 +528,28 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         __syncwarp();
     } else if (warp < 3 + kNvPairCopiers) {
         // ---------------------------------------------------------------- scale copiers (leader CTA only)
-        // Copier w moves word w of the three scale blocks.  Slot `stage` is free when the stage's "full" barrier
-        // fires: the MMAs that read it completed before the producers were allowed to refill the stage.
+        // Copier w moves word w of the scale blocks.  Slot `stage` is free when the stage's "full" barrier fires: the
+        // MMAs that read it completed before the producers were allowed to refill the stage.
         const uint32_t w = warp - 3;
         if (lane == 0 && cta_rank == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
+                const bool two = get(idx).cols > 128;
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_full + stage * 8, phase, s_abort, p.status, kDevTimeoutConvert);
                     if (!ok) {
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t ssf = ring + stage * S::kStageBytes + S::kABytes + S::kBBytes + w * 512;
-                    const uint32_t t_sfa = tmem_base + kAccCols + stage * kSfSlot;
-                    const uint32_t t_sfb = t_sfa + 16 + w * 8;
-                    tmem_cp_32x128b_warpx4_pair(t_sfa + w * 4, make_smem_desc_noswizzle(ssf, 16, 128));
-                    tmem_cp_32x128b_warpx4_pair(t_sfb, make_smem_desc_noswizzle(ssf + 2048, 16, 128));
-                    tmem_cp_32x128b_warpx4_pair(t_sfb + 4, make_smem_desc_noswizzle(ssf + 4096, 16, 128));
+                    const uint32_t ssf = ring + stage * S::kStageBytes + S::kWBytes + S::kXBytes + w * 512;
+                    const uint32_t t_sfw = tmem_base + kAccCols + stage * kSfSlot;
+                    const uint32_t t_sfx = t_sfw + 16 + w * 8;
+                    tmem_cp_32x128b_warpx4_pair(t_sfw + w * 4, make_smem_desc_noswizzle(ssf, 16, 128));
+                    tmem_cp_32x128b_warpx4_pair(t_sfx, make_smem_desc_noswizzle(ssf + 2048, 16, 128));
+                    if (two) {
+                        tmem_cp_32x128b_warpx4_pair(t_sfx + 4, make_smem_desc_noswizzle(ssf + 4096, 16, 128));
+                    }
                     umma_commit<2>(bar_sf_full + stage * 8);
                     if (++stage == kStages) {
                         stage = 0;
@@ -606,66 +562,50 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     } else {
         // ---------------------------------------------------------------- epilogue: sixteen warps per CTA
         const uint32_t quad = warp & 3;                           // TMEM lane quarter this warp may read
-        const uint32_t part = (warp - 3 - kNvPairCopiers) >> 2;   // which 64 columns of the tile's 256
-        const bool staged = (p.n & (p.d_type == 0 ? 3u : 7u)) != 0;
-        uint8_t* slab = smem + S::kSlabOffset +
-                        (warp - 3 - kNvPairCopiers) * (staged ? S::kOddSlabBytes : S::kSlabBytes);
+        const uint32_t part = (warp - 3 - kNvPairCopiers) >> 2;   // which 64 rows of A
+        uint8_t* slab = smem + S::kRingBytes + (warp - 3 - kNvPairCopiers) * S::kSlabBytes;
         uint32_t acc_phase = 0;
         bool ok = true;
         for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
-            uint32_t mt, nt;
-            mx_tile_coords(idx, m_tiles, n_tiles, p.band_rows, mt, nt);
-            int32_t tile_row0, row_end, group;
-            row_tile(mt, tile_row0, row_end, group);
-            const float alpha = p.alpha != nullptr ? __ldg(p.alpha + group) : 1.0f;
+            const Tile t = get(idx);
+            const float alpha = p.alpha != nullptr ? __ldg(p.alpha + t.group) : 1.0f;
             ok = mbar_wait(bar_tmem_full, acc_phase, s_abort, p.status, kDevTimeoutEpilogue);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
                 break;
             }
             tcgen05_fence_after();
-            const uint32_t taddr = tmem_base + part * 64 + ((quad * 32u) << 16);
+            const uint32_t first = part * 64;
+            const uint32_t rows = t.rows > first ? t.rows - first : 0u;  // of this warp's 64
+            const uint32_t taddr = tmem_base + first + ((quad * 32u) << 16);
             uint32_t r[2][32];
-            tmem_ld_32x32b_x32(taddr, r[0]);
-            tmem_ld_32x32b_x32(taddr + 32, r[1]);
-            tmem_ld_wait();
+            if (rows != 0) {
+                tmem_ld_32x32b_x32(taddr, r[0]);
+                tmem_ld_32x32b_x32(taddr + 32, r[1]);
+                tmem_ld_wait();
+            }
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive_cluster(bar_tmem_empty, 0);  // this warp's share is in registers
             }
             acc_phase ^= 1;
-            const uint32_t row0 = static_cast<uint32_t>(tile_row0) + cta_rank * kBlockM + quad * 32, row = row0 + lane;
-            const uint32_t col = nt * kMxBlockN + part * 64;
-            if (col >= p.n || row0 >= static_cast<uint32_t>(row_end)) {
+            const uint32_t col0 = t.nt * kNvTileW + cta_rank * 128 + quad * 32;
+            if (col0 >= p.n) {
                 continue;
             }
-            if (staged) {
-                uint32_t* words = reinterpret_cast<uint32_t*>(slab);
-                nv_store_rows_staged(p, r[0], words, row0, static_cast<uint32_t>(row_end), col, alpha, lane);
-                if (col + 32 < p.n) {
-                    nv_store_rows_staged(p, r[1], words, row0, static_cast<uint32_t>(row_end), col + 32, alpha, lane);
-                }
-            } else if (p.tma_store && row0 + 32 <= static_cast<uint32_t>(row_end)) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t row0 = t.row0 + first + h * 32;
+                if (p.tma_store && rows >= h * 32 + 32u) {
                     if (p.d_type == 0) {
-#pragma unroll
-                        for (int f = 0; f < 2; ++f) {
-                            if (col + h * 32 + f * 16 < p.n) {
-                                nv_slab_free(lane);
-                                nv_tma_store<16>(p, &tmap_d, r[h] + f * 16, slab, row0, col + h * 32 + f * 16, alpha, lane);
-                            }
-                        }
-                    } else if (col + h * 32 < p.n) {
-                        nv_slab_free(lane);
-                        nv_tma_store<32>(p, &tmap_d, r[h], slab, row0, col + h * 32, alpha, lane);
+                        nv_tma_store_columns<16>(p, &tmap_d, r[h], slab, row0, col0, alpha, lane);
+                        nv_tma_store_columns<16>(p, &tmap_d, r[h] + 16, slab, row0 + 16, col0, alpha, lane);
+                    } else {
+                        nv_tma_store_columns<32>(p, &tmap_d, r[h], slab, row0, col0, alpha, lane);
                     }
-                }
-            } else if (row < static_cast<uint32_t>(row_end)) {
-                nv_store_row<32>(p, r[0], row, col, alpha);
-                if (col + 32 < p.n) {
-                    nv_store_row<32>(p, r[1], row, col + 32, alpha);
+                } else if (rows > h * 32u) {
+                    nv_store_columns<32>(p, r[h], row0, rows - h * 32, col0 + lane, alpha);
                 }
             }
         }
