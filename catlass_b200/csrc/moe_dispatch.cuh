@@ -106,12 +106,18 @@ moe_count_kernel(const DispatchParams p)
         s_count[e] = 0;
     }
     __syncthreads();
-    const uint32_t begin = blockIdx.x * p.chunk;
-    for (uint32_t i = threadIdx.x; i < p.chunk; i += kDispatchThreads) {
-        if (begin + i < p.pairs) {
-            const uint32_t e = dispatch_expert(p, begin + i);
-            if (e < p.experts) {
-                atomicAdd(s_count + e, 1u);
+    const uint32_t begin = blockIdx.x * p.chunk + threadIdx.x;
+    for (uint32_t i = 0; i < p.chunk; i += 4 * kDispatchThreads) {
+        uint32_t e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // (four loads in flight)
+            const uint32_t pair = begin + i + u * kDispatchThreads;
+            e[u] = i + u * kDispatchThreads < p.chunk && pair < p.pairs ? dispatch_expert(p, pair) : p.experts;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (e[u] < p.experts) {
+                atomicAdd(s_count + e[u], 1u);
             }
         }
     }
@@ -139,32 +145,60 @@ moe_place_kernel(const DispatchParams p)
     const uint32_t per_warp = p.chunk / kDispatchWarps;
     const uint32_t begin = blockIdx.x * p.chunk + warp * per_warp;
     uint32_t* mine = s_warp + warp * p.experts;
-    for (uint32_t i = lane; i < per_warp; i += 32) {
-        if (begin + i < p.pairs) {
-            const uint32_t e = dispatch_expert(p, begin + i);
-            if (e < p.experts) {
-                atomicAdd(mine + e, 1u);
+    for (uint32_t i = 0; i < per_warp; i += 128) {
+        uint32_t e[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t at = i + u * 32 + lane;
+            e[u] = at < per_warp && begin + at < p.pairs ? dispatch_expert(p, begin + at) : p.experts;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            if (e[u] < p.experts) {
+                atomicAdd(mine + e[u], 1u);
             }
         }
     }
+    for (uint32_t e = threadIdx.x; e < p.experts; e += kDispatchThreads) {
+        s_first[e] = 0;
+        s_before[e] = 0;
+    }
     __syncthreads();
     grid_dependency_wait();  // the chunks' counts
-    for (uint32_t e = threadIdx.x; e < p.experts; e += kDispatchThreads) {
-        uint32_t before = 0, total = 0;
-        if (p.chunks == 1) {
+    if (p.chunks == 1) {
+        for (uint32_t e = threadIdx.x; e < p.experts; e += kDispatchThreads) {
+            uint32_t total = 0;
             for (int w = 0; w < kDispatchWarps; ++w) {
                 total += s_warp[w * p.experts + e];
             }
-        } else {
-#pragma unroll 8
-            for (uint32_t c = 0; c < p.chunks; ++c) {
-                const uint32_t v = p.counts[static_cast<size_t>(c) * p.experts + e];
-                total += v;
-                before += c < blockIdx.x ? v : 0u;
-            }
+            s_first[e] = total;
         }
-        s_first[e] = total;
-        s_before[e] = before;
+    } else {
+        // Sums of an expert's counts over all chunks and over those in front: a column of the table is shared by as many
+        // threads as there are (one thread per expert walking 128 chunks took 5 us), eight loads of each in flight.
+        uint32_t wide = 32;
+        while (wide < p.experts && wide < kDispatchThreads) {
+            wide *= 2;
+        }
+        const uint32_t parts = kDispatchThreads / wide, part = threadIdx.x / wide;
+        for (uint32_t e = threadIdx.x % wide; e < p.experts; e += wide) {
+            uint32_t before = 0, total = 0;
+            for (uint32_t c0 = part; c0 < p.chunks; c0 += 8 * parts) {
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const uint32_t c = c0 + u * parts;
+                    v[u] = c < p.chunks ? p.counts[static_cast<size_t>(c) * p.experts + e] : 0u;
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    total += v[u];
+                    before += c0 + u * parts < blockIdx.x ? v[u] : 0u;
+                }
+            }
+            atomicAdd(s_first + e, total);  // (integers: the order does not matter)
+            atomicAdd(s_before + e, before);
+        }
     }
     __syncthreads();
     if (warp == 0) {
@@ -311,18 +345,24 @@ moe_rows_kernel(const DispatchParams p)
             }
         }
         __syncthreads();
-    } else {
-        grid_dependency_wait();
-        if (threadIdx.x < p.top_k) {
-            s_row[threadIdx.x] = p.position[static_cast<uint64_t>(token) * p.top_k + threadIdx.x];
-        }
-        __syncthreads();
     }
+    // The rows of this token's pairs.  In front of the wait x may be read (it was complete before the count kernel
+    // started), nothing may be written.
+    auto rows_known = [&]() {
+        if constexpr (!kFused) {
+            grid_dependency_wait();
+            if (threadIdx.x < p.top_k) {
+                s_row[threadIdx.x] = p.position[static_cast<uint64_t>(token) * p.top_k + threadIdx.x];
+            }
+            __syncthreads();
+        }
+    };
     if constexpr (kFormat == kRowsIndex) {
         return;
     }
     const uint8_t* xr = static_cast<const uint8_t*>(p.x) + token * p.x_pitch * kElemBytes;
     if constexpr (kFormat == kRowsCopy) {
+        rows_known();
         const uint32_t vecs = p.k * kElemBytes / 16;
         for (uint32_t c = threadIdx.x; c < vecs; c += kDispatchThreads) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(xr) + c);
@@ -357,19 +397,30 @@ moe_rows_kernel(const DispatchParams p)
             amax = fmaxf(amax, s_max[w]);
         }
         inv = amax > 0.0f ? __fdiv_rn(127.0f, amax) : 0.0f;
+        rows_known();
         if (threadIdx.x < p.top_k && s_row[threadIdx.x] >= 0) {
             static_cast<float*>(p.scale)[s_row[threadIdx.x]] = __fdiv_rn(amax, 127.0f);
         }
     }
     const float tensor_scale = kFormat == kRowsNvfp4 ? __ldg(p.tensor_scale) : 0.0f;
     const uint32_t ks = (p.k / 32 + 1u) & ~1u;
+    Raw16<kType> raw;
+    if (threadIdx.x < blocks) {
+        raw.load(xr, static_cast<uint64_t>(threadIdx.x) * 16);
+    }
+    if constexpr (kFormat != kRowsInt8) {
+        rows_known();
+    }
     // (the same trips for every lane: the maximum of an MX block is exchanged between the two lanes that share it)
     for (uint32_t c0 = 0; c0 < blocks; c0 += kDispatchThreads) {
         const uint32_t c = c0 + threadIdx.x;
         const bool active = c < blocks;
         float v[16];
         if (active) {
-            load_vec<kType, 16>(xr, static_cast<uint64_t>(c) * 16, v);
+            raw.floats(v);
+            if (c + kDispatchThreads < blocks) {
+                raw.load(xr, static_cast<uint64_t>(c + kDispatchThreads) * 16);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
