@@ -237,29 +237,47 @@ int cb200_moe_route(const cb200_moe_route_args* a, void* stream_v)
     p.weights = a->weights;
     p.ids = a->ids;
     p.score_needed = a->bias != nullptr || (p.groups > 1 && p.group_top2) ? 1u : 0u;
+    // lanes that hold a group when every lane has `per` experts; 0: groups are not whole lanes
+    auto group_lanes = [&](uint32_t per) {
+        const uint32_t lanes = p.per_group / per;
+        return p.per_group % per == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0u;
+    };
     uint32_t per = 1;  // logits per lane: 1, 2, 4 ... 32
     while (per * 32u < a->experts) {
         per *= 2;
     }
+    const uint32_t per_many = a->experts <= 64u ? 8u : (a->experts <= 128u ? 16u : 32u);
+    const uint32_t lanes_many = p.groups == 1u ? 8u : group_lanes(per_many);
+    const bool many = a->tokens >= kRouteManyTokens && a->top_k <= 8u && a->experts > 16u && a->experts <= 256u &&
+                      lanes_many != 0 && lanes_many * p.groups <= 8u * (p.groups == 1u ? 8u : 1u);
+    per = many ? per_many : per;
     const uint64_t share = per * float_bytes(a->logits_type);  // bytes of a lane's logits
     const uint64_t step = share < 16u ? share : 16u;
     p.vector = (p.pitch * float_bytes(a->logits_type)) % step == 0 && aligned_to(a->logits, step) ? 1u : 0u;
-    const uint32_t lanes = p.per_group / per;
-    p.group_lanes = p.per_group % per == 0 && (lanes & (lanes - 1)) == 0 && lanes * p.groups <= 32u ? lanes : 0u;
+    p.group_lanes = many ? lanes_many : (group_lanes(per) * p.groups <= 32u ? group_lanes(per) : 0u);
     p.walk_lanes = 32;
     while (p.walk_lanes * p.groups > 32u) {
         p.walk_lanes /= 2;
     }
-    const uint32_t grid = (a->tokens + kRouteWarps - 1) / kRouteWarps;
+    const uint32_t per_cta = many ? kRouteWarps * 4u : kRouteWarps;  // tokens
+    const uint32_t grid = (a->tokens + per_cta - 1) / per_cta;
     const uint32_t smem = kRouteWarps * a->experts * 8u;
     const uint32_t threads = kRouteWarps * 32;
-    switch (per) {
-        case 1: moe_route_kernel<1><<<grid, threads, smem, stream>>>(p); break;
-        case 2: moe_route_kernel<2><<<grid, threads, smem, stream>>>(p); break;
-        case 4: moe_route_kernel<4><<<grid, threads, smem, stream>>>(p); break;
-        case 8: moe_route_kernel<8><<<grid, threads, smem, stream>>>(p); break;
-        case 16: moe_route_kernel<16><<<grid, threads, smem, stream>>>(p); break;
-        default: moe_route_kernel<32><<<grid, threads, smem, stream>>>(p); break;
+    if (many) {
+        switch (per) {
+            case 8: moe_route_many_kernel<8><<<grid, threads, smem, stream>>>(p); break;
+            case 16: moe_route_many_kernel<16><<<grid, threads, smem, stream>>>(p); break;
+            default: moe_route_many_kernel<32><<<grid, threads, smem, stream>>>(p); break;
+        }
+    } else {
+        switch (per) {
+            case 1: moe_route_kernel<1><<<grid, threads, smem, stream>>>(p); break;
+            case 2: moe_route_kernel<2><<<grid, threads, smem, stream>>>(p); break;
+            case 4: moe_route_kernel<4><<<grid, threads, smem, stream>>>(p); break;
+            case 8: moe_route_kernel<8><<<grid, threads, smem, stream>>>(p); break;
+            case 16: moe_route_kernel<16><<<grid, threads, smem, stream>>>(p); break;
+            default: moe_route_kernel<32><<<grid, threads, smem, stream>>>(p); break;
+        }
     }
     CB200_CUDA_TRY(cudaGetLastError());
     g_launches.fetch_add(1, std::memory_order_relaxed);

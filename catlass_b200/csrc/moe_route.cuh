@@ -23,6 +23,10 @@
 
 namespace cb200 {
 
+// From so many tokens on four of them share a warp, where the experts allow it.  256 experts in 8 groups with a bias, one /
+// four tokens per warp: 512 tokens 4.7 / 6.4 us, 4096 7.9 / 7.9, 16384 23 / 16, 131072 144 / 96; 60 experts: 512 3.6 / 4.2,
+// 4099 4.6 / 4.5, 16384 10.6 / 8.1.
+constexpr uint32_t kRouteManyTokens = 4096;
 constexpr int kRouteWarps = 4;  // tokens per CTA: small, so that a few tokens spread over the SMs
 
 struct RouteParams {
@@ -152,96 +156,108 @@ __device__ __forceinline__ uint32_t route_keep_groups(F key, uint32_t groups, ui
     return mask;
 }
 
-// The token's selection with 64-bit keys.  keys: shared memory of this warp, one double per expert.  Lane j receives
-// the id of slot j in `id`; returns the number of slots filled.
+// Unsigned integers in the order of the doubles, 0 below them all.
+__device__ __forceinline__ unsigned long long route_order64(double f)
+{
+    const unsigned long long b = __double_as_longlong(f);
+    return b ^ (static_cast<unsigned long long>(static_cast<long long>(b) >> 63) | 0x8000000000000000ull);
+}
+
+// The token's selection with 64-bit keys, kPer experts (i * 32 + lane) per lane.  keys: shared memory of this warp, one
+// double per expert, for the groups' walk.  Lane j receives the id of slot j in `id`; returns the number of slots filled.
+template <int kPer>
 __device__ __noinline__ uint32_t route_select_exact(const RouteParams& p, uint32_t token, double* keys, uint32_t lane,
                                                     int32_t* id)
 {
+    constexpr uint32_t kAll = 0xffffffffu;
     const double kMinusInf = -CUDART_INF;
-    float max = -CUDART_INF_F;
-    double total = 1.0;
-    if (p.softmax) {
-        for (uint32_t e = lane; e < p.experts; e += 32) {
-            max = fmaxf(max, route_logit(p, token, e));
-        }
+    float x[kPer];
+    double s[kPer], key[kPer];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            max = fmaxf(max, __shfl_xor_sync(0xffffffffu, max, off));
-        }
-        double sum = 0.0;
-        for (uint32_t e = lane; e < p.experts; e += 32) {
-            const float x = route_logit(p, token, e);
-            sum += x == max ? 1.0 : exp(static_cast<double>(x) - static_cast<double>(max));
-        }
-        total = warp_sum64(sum);
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t e = i * 32 + lane;
+        x[i] = e < p.experts ? route_logit(p, token, e) : -CUDART_INF_F;
     }
-    auto score = [&](float x) -> double {
-        if (p.softmax) {
-            return (x == max ? 1.0 : exp(static_cast<double>(x) - static_cast<double>(max))) / total;
+    if (p.softmax) {
+        float max = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            max = fmaxf(max, x[i]);
         }
-        return 1.0 / (1.0 + exp(-static_cast<double>(x)));
-    };
-    // keys[] by what decides: the groups' values first, then (the same unless groups go by score and experts by logit)
-    // the experts' keys
-    auto fill = [&](bool for_groups) {
-        for (uint32_t e = lane; e < p.experts; e += 32) {
-            const float x = route_logit(p, token, e);
-            double v = kMinusInf;
-            if (x > -CUDART_INF_F) {
-                v = p.bias != nullptr ? score(x) + static_cast<double>(p.bias[e])
-                                      : (for_groups && p.group_top2 ? score(x) : static_cast<double>(x));
-            }
-            keys[e] = v > kMinusInf ? v : kMinusInf;
+        max = route_unorder(__reduce_max_sync(kAll, route_order(max)));
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] = x[i] == max ? 1.0 : exp(static_cast<double>(x[i]) - static_cast<double>(max));
+            sum += s[i];
         }
-    };
-    __syncwarp();
-    fill(p.groups > 1);
+        sum = warp_sum64(sum);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] /= sum;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t e = i * 32 + lane;
+        key[i] = p.bias == nullptr ? static_cast<double>(x[i])
+                                   : s[i] + static_cast<double>(e < p.experts ? p.bias[e] : 0.0f);
+        key[i] = x[i] > -CUDART_INF_F && key[i] > kMinusInf ? key[i] + 0.0 : kMinusInf;
+    }
     if (p.groups > 1) {
+        const bool by_score = p.bias == nullptr && p.group_top2;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t e = i * 32 + lane;
+            if (e < p.experts) {
+                keys[e] = by_score ? (key[i] > kMinusInf ? s[i] : kMinusInf) : key[i];
+            }
+        }
         __syncwarp();
         const double g = route_group_key<double>(keys, p.groups, p.per_group, p.walk_lanes, lane, p.group_top2 != 0,
                                                  kMinusInf);
         const uint32_t keep = route_keep_groups<double>(g, p.groups, p.groups_kept, p.walk_lanes, lane);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t of = (i * 32 + lane) / p.per_group;
+            key[i] = of < p.groups && ((keep >> of) & 1u) != 0 ? key[i] : kMinusInf;
+        }
         __syncwarp();
-        if (p.bias == nullptr && p.group_top2) {
-            fill(false);
-        }
-        for (uint32_t e = lane; e < p.experts; e += 32) {
-            if (((keep >> (e / p.per_group)) & 1u) == 0) {
-                keys[e] = kMinusInf;
-            }
-        }
     }
     uint32_t filled = 0;
     for (uint32_t j = 0; j < p.top_k; ++j) {
         double best = kMinusInf;
-        uint32_t at = 0xffffffffu;
-        for (uint32_t e = lane; e < p.experts; e += 32) {  // (each lane reads and clears its own experts only)
-            if (keys[e] > best) {
-                best = keys[e];
-                at = e;
-            }
-        }
+        uint32_t at = 0;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            const double b = __shfl_xor_sync(0xffffffffu, best, off);
-            const uint32_t a = __shfl_xor_sync(0xffffffffu, at, off);
-            if (b > best || (b == best && a < at)) {
-                best = b;
-                at = a;
+        for (int i = 0; i < kPer; ++i) {
+            if (key[i] > best) {
+                best = key[i];
+                at = i * 32 + lane;
             }
         }
-        if (at == 0xffffffffu) {
+        const unsigned long long order = best > kMinusInf ? route_order64(best) : 0ull;
+        const uint32_t high = __reduce_max_sync(kAll, static_cast<uint32_t>(order >> 32));
+        if (high == 0) {  // (a finite key is above 2^52 in this order)
             break;
         }
-        if (at % 32 == lane) {
-            keys[at] = kMinusInf;
+        const bool still = static_cast<uint32_t>(order >> 32) == high;
+        const uint32_t low = __reduce_max_sync(kAll, still ? static_cast<uint32_t>(order) : 0u);
+        at = __reduce_min_sync(kAll, still && static_cast<uint32_t>(order) == low ? at : kAll);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            key[i] = i * 32 + lane == at ? kMinusInf : key[i];
         }
         if (lane == j) {
             *id = static_cast<int32_t>(at);
         }
         ++filled;
     }
-    __syncwarp();
     return filled;
 }
 
@@ -573,7 +589,7 @@ moe_route_kernel(const __grid_constant__ RouteParams p)
             }
             if (redo) {
                 my_id = -1;
-                filled = route_select_exact(p, token, route_smem + warp * p.experts, lane, &my_id);
+                filled = route_select_exact<kPer>(p, token, route_smem + warp * p.experts, lane, &my_id);
             }
         }
         float w = 0.0f;
@@ -594,6 +610,354 @@ moe_route_kernel(const __grid_constant__ RouteParams p)
             p.ids[at] = lane < filled ? my_id : -1;
             p.weights[at] = lane < filled ? w : 0.0f;
         }
+    }
+}
+
+// ---------------------------------------------------------------- many tokens: four per warp
+//
+// Eight lanes share a token, kPer experts each: reductions take three shuffles for four tokens at once, and the instructions
+// of a token's selection, what the kernel above spends most of its time on, are shared by four.  At most 8 experts per
+// token, 256 in all; groups are whole lanes, a power of two of them each.  What is in doubt is settled in place, by the
+// candidates' keys in 64 bits; the rest goes to route_select_exact, a token at a time.
+
+// a and b sorted descending: a becomes the eight largest of both, sorted; returns the largest of the others
+__device__ __forceinline__ uint32_t merge_top8(uint32_t (&a)[8], const uint32_t (&b)[8])
+{
+    uint32_t rest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t x = a[i], y = b[7 - i];
+        a[i] = x > y ? x : y;
+        const uint32_t low = x > y ? y : x;
+        rest = low > rest ? low : rest;
+    }
+#pragma unroll
+    for (int k = 4; k >= 1; k >>= 1) {  // (a is bitonic now)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if ((i & k) == 0) {
+                const uint32_t x = a[i], y = a[i + k];
+                a[i] = x > y ? x : y;
+                a[i + k] = x > y ? y : x;
+            }
+        }
+    }
+    return rest;
+}
+
+// Dynamic shared memory: kRouteWarps * experts doubles.
+template <int kPer>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+moe_route_many_kernel(const __grid_constant__ RouteParams p)
+{
+    extern __shared__ double route_smem[];
+    static_assert(kPer == 8 || kPer == 16 || kPer == 32, "experts per lane");
+    constexpr uint32_t kAll = 0xffffffffu;
+    constexpr uint32_t kLow = kPer - 1;
+    const float kMinusInf = -CUDART_INF_F;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t sub = lane & 7u, base = lane & 24u;       // lane of the token, first lane of the token
+    const uint32_t first_token = (blockIdx.x * kRouteWarps + warp) * 4;
+    if (first_token >= p.tokens) {
+        return;
+    }
+    const uint32_t token = first_token + (lane >> 3);
+    const uint32_t e0 = sub * kPer;
+    const bool exact_keys = p.bias == nullptr;
+    const bool active = token < p.tokens && (p.token_count == nullptr ||
+                                             static_cast<int64_t>(token) < static_cast<int64_t>(*p.token_count));
+    float x[kPer], s[kPer], key[kPer];
+    if (active) {
+        route_load<kPer>(p, token, e0, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            x[i] = kMinusInf;
+        }
+    }
+    bool numbers = e0 + kPer <= p.experts;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        key[i] = !exact_keys && e0 + i < p.experts ? __ldg(p.bias + e0 + i) : 0.0f;
+        numbers = numbers && x[i] > kMinusInf && key[i] > kMinusInf;
+    }
+    const bool clean = __all_sync(kAll, numbers);
+    if (!clean) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            x[i] = x[i] > kMinusInf && key[i] > kMinusInf ? x[i] : kMinusInf;
+        }
+    }
+    float max = kMinusInf, inv_total = 1.0f;
+    if (p.softmax) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            max = fmaxf(max, x[i]);
+        }
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) {
+            max = fmaxf(max, __shfl_xor_sync(kAll, max, off));
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] = route_exp_diff(x[i], max);
+            sum += s[i];
+        }
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) {
+            sum += __shfl_xor_sync(kAll, sum, off);
+        }
+        inv_total = __frcp_rn(sum);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] *= inv_total;
+        }
+    } else if (p.score_needed) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s[i] = route_sigmoid_fast(x[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        key[i] = exact_keys ? x[i] + 0.0f : s[i] + key[i];
+    }
+    if (!clean) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            key[i] = x[i] > kMinusInf ? key[i] : kMinusInf;
+        }
+    }
+    // (the same distances as in the kernel above, which derives them)
+    const float apart = p.softmax ? inv_total * 0x1p-17f : 0x1p-20f;
+    constexpr float kRounding = 0x1p-22f + kPer * 0x1p-23f;
+    // a lane's eight largest, sorted, and the largest of its others
+    uint32_t list[8], rest = 0;
+    {
+        uint32_t part[kPer / 8][8];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t o = (route_order(key[i]) & ~kLow) | (kLow - i);
+            part[i / 8][i % 8] = !clean && !(key[i] > kMinusInf) ? 0u : o;
+        }
+#pragma unroll
+        for (int h = 0; h < kPer / 8; ++h) {
+            sort_descending<8>(part[h]);
+        }
+        if constexpr (kPer == 32) {
+            const uint32_t r0 = merge_top8(part[0], part[1]), r1 = merge_top8(part[2], part[3]);
+            rest = merge_top8(part[0], part[2]);
+            rest = rest > r0 ? rest : r0;
+            rest = rest > r1 ? rest : r1;
+        } else if constexpr (kPer == 16) {
+            rest = merge_top8(part[0], part[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            list[i] = part[0][i];
+        }
+    }
+    // a key in 64 bits (softmax scores without the common divisor)
+    auto exact_key = [&](uint32_t e, bool by_score) -> double {
+        const float logit = route_logit(p, token, e);
+        if (exact_keys && !by_score) {
+            return static_cast<double>(logit);
+        }
+        if (p.softmax) {
+            return logit == max ? 1.0 : exp(static_cast<double>(logit) - static_cast<double>(max));
+        }
+        return 1.0 / (1.0 + exp(-static_cast<double>(logit))) + (exact_keys ? 0.0 : static_cast<double>(p.bias[e]));
+    };
+    bool redo = false;  // the whole token again in 64 bits
+    if (p.groups > 1) {
+        const bool by_score = exact_keys && p.group_top2;
+        float g = kMinusInf, second = kMinusInf;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const float v = by_score ? (key[i] > kMinusInf ? s[i] : kMinusInf) : key[i];
+            second = fmaxf(second, fminf(g, v));
+            g = fmaxf(g, v);
+        }
+        for (uint32_t off = 1; off < p.group_lanes; off <<= 1) {
+            const float f = __shfl_xor_sync(kAll, g, off), u = __shfl_xor_sync(kAll, second, off);
+            second = fmaxf(fminf(g, f), fmaxf(second, u));
+            g = fmaxf(g, f);
+        }
+        g = p.group_top2 && second > kMinusInf ? g + second : g;
+        const uint32_t mine = sub / p.group_lanes;
+        uint32_t rank = 0;
+        for (uint32_t h = 0; h < p.groups; ++h) {
+            const float other = __shfl_sync(kAll, g, base + h * p.group_lanes);
+            rank += (other > g || (other == g && h < mine)) ? 1u : 0u;
+        }
+        const bool is_group = mine < p.groups;
+        bool shut = !is_group || rank >= p.groups_kept;
+        if (p.score_needed) {
+            float low = shut ? CUDART_INF_F : g, high = is_group && shut ? g : kMinusInf;
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) {
+                low = fminf(low, __shfl_xor_sync(kAll, low, off));
+                high = fmaxf(high, __shfl_xor_sync(kAll, high, off));
+            }
+            redo = high > kMinusInf && low - high <= 2.0f * apart + 0x1p-21f * fabsf(low);
+        }
+        if (__any_sync(kAll, redo)) {
+            // The groups' keys of such a token in 64 bits: where a group is one lane, from the two largest of its list,
+            // unless its third may belong to them.  (What cannot be settled so stays to be redone.)
+            bool settled = p.group_lanes == 1 && !(p.softmax && !exact_keys);
+            double g64 = -CUDART_INF;
+            if (redo && settled && list[0] != 0) {
+                const uint32_t e1 = e0 + (kLow - (list[0] & kLow)), e2 = e0 + (kLow - (list[1] & kLow));
+                const double k1 = exact_key(e1, by_score), k2 = list[1] != 0 ? exact_key(e2, by_score) : -CUDART_INF;
+                g64 = p.group_top2 && list[1] != 0 ? k1 + k2 : (k1 > k2 ? k1 : k2);
+                if (list[2] != 0) {  // (the logits' own order is exact but for the bits that hold their place)
+                    const float a = route_unorder(list[1] & ~kLow), b = route_unorder(list[2] & ~kLow);
+                    settled = a - b > (exact_keys ? 0.0f : apart) + kRounding * fabsf(a);
+                }
+            }
+            settled = ((__ballot_sync(kAll, settled) >> base) & 0xffu) == 0xffu;
+            uint32_t rank64 = 0;
+            for (uint32_t h = 0; h < p.groups; ++h) {
+                const double other = __shfl_sync(kAll, g64, (base + h * p.group_lanes) & 31u);
+                rank64 += (other > g64 || (other == g64 && h < mine)) ? 1u : 0u;
+            }
+            if (redo && settled) {
+                shut = !is_group || rank64 >= p.groups_kept;
+                redo = false;
+            }
+        }
+        if (shut) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                list[i] = 0u;
+            }
+            rest = 0u;
+        }
+    }
+    // One expert after the other: the largest of the lanes' first keys, of equal ones the lowest lane's; slot j in lane j.
+    uint32_t filled = 0, taken = 0, taken_id = 0;
+    uint32_t top = 0, from = 0;
+    auto look = [&]() {  // top: the largest first key without its place (0: none left); from: its lane
+        top = list[0] & ~kLow;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) {
+            const uint32_t other = __shfl_xor_sync(kAll, top, off);
+            top = other > top ? other : top;
+        }
+        const uint32_t at = (__ballot_sync(kAll, (list[0] & ~kLow) == top) >> base) & 0xffu;
+        from = __ffs(at) - 1;  // (at least the lane of the maximum)
+    };
+    for (uint32_t j = 0; j < p.top_k; ++j) {
+        look();
+        const uint32_t value = __shfl_sync(kAll, list[0], base + from);
+        if (sub == j) {
+            taken = value;
+            taken_id = from * kPer + (kLow - (value & kLow));
+        }
+        filled += top != 0 ? 1u : 0u;
+        const bool owner = sub == from;
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+            list[i] = owner ? list[i + 1] : list[i];
+        }
+        list[7] = owner ? rest : list[7];
+        rest = owner ? 0u : rest;
+    }
+    // Two neighbours in the order, the last of them the best that is not taken, may be the other way round unless they are
+    // clearly apart or the same logit with the same bias.
+    look();
+    const uint32_t next = __shfl_sync(kAll, list[0], base + from);
+    const uint32_t next_id = from * kPer + (kLow - (next & kLow));
+    uint32_t below = __shfl_down_sync(kAll, taken, 1), below_id = __shfl_down_sync(kAll, taken_id, 1);
+    below = sub + 1 == p.top_k ? next : below;
+    below_id = sub + 1 == p.top_k ? next_id : below_id;
+    auto near = [&](uint32_t above, uint32_t here) {
+        if (exact_keys) {  // logits: only those that agree in all bits that were kept; two-byte ones are then the same
+            return p.logits_type == 0 && (above & ~kLow) - (here & ~kLow) <= kPer;
+        }
+        const float a = route_unorder(above & ~kLow), b = route_unorder(here & ~kLow);
+        return a - b <= apart + kRounding * fabsf(a);
+    };
+    bool close = false;
+    const bool last = sub + 1 == p.top_k;
+    if (sub < p.top_k && sub < filled && (last ? top != 0 : sub + 1 < filled)) {
+        close = near(taken, below);
+    }
+    const bool edge = last && close;  // the next best may belong to the taken ones, and what comes behind it too
+    if (close) {
+        close = route_logit(p, token, taken_id) != route_logit(p, token, below_id) ||
+                (!exact_keys && p.bias[taken_id] != p.bias[below_id]);
+    }
+    int32_t my_id = sub < filled ? static_cast<int32_t>(taken_id) : -1;
+    if (__any_sync(kAll, close || edge)) {
+        // The keys of the taken ones and of the next best in 64 bits, and their order by those.  That settles a token unless
+        // more than the next best are in question, or the softmax total would be needed in 64 bits.
+        const uint32_t mine = (__ballot_sync(kAll, close) >> base) & 0xffu;
+        const bool border = ((__ballot_sync(kAll, edge) >> base) & 0xffu) != 0;
+        const bool owner = sub == from;
+        const uint32_t behind = owner ? list[1] : list[0];
+        bool more = behind != 0 ? near(next, behind) : kPer > 8 && owner;  // (nothing known behind the next best)
+        more = ((__ballot_sync(kAll, more) >> base) & 0xffu) != 0;
+        if ((border && more) || (mine != 0 && p.softmax && !exact_keys)) {
+            redo = true;
+        }
+        double key64 = -CUDART_INF, next64 = -CUDART_INF;
+        if (mine != 0 && sub < filled) {
+            key64 = exact_key(taken_id, false);
+        }
+        if (mine != 0 && border) {
+            next64 = exact_key(next_id, false);
+        }
+        uint32_t rank = border && (next64 > key64 || (next64 == key64 && next_id < taken_id)) ? 1u : 0u;
+        uint32_t next_rank = 0;
+        for (uint32_t h = 0; h < p.top_k; ++h) {
+            const double other = __shfl_sync(kAll, key64, base + h);
+            const uint32_t other_id = __shfl_sync(kAll, taken_id, base + h);
+            if (h < filled) {
+                rank += (other > key64 || (other == key64 && other_id < taken_id)) ? 1u : 0u;
+                next_rank += (other > next64 || (other == next64 && other_id < next_id)) ? 1u : 0u;
+            }
+        }
+        int32_t id = border && next_rank == sub ? static_cast<int32_t>(next_id) : -1;
+        for (uint32_t h = 0; h < p.top_k; ++h) {
+            const uint32_t to = __shfl_sync(kAll, rank, base + h), other_id = __shfl_sync(kAll, taken_id, base + h);
+            id = h < filled && to == sub ? static_cast<int32_t>(other_id) : id;
+        }
+        my_id = mine != 0 && sub < filled ? id : my_id;
+    }
+    const uint32_t again = __ballot_sync(kAll, redo);
+    if (again != 0) {
+        for (uint32_t t = 0; t < 4; ++t) {
+            if (((again >> (8 * t)) & 0xffu) != 0) {
+                int32_t id = -1;
+                const uint32_t n = route_select_exact<8>(p, first_token + t, route_smem + warp * p.experts, lane, &id);
+                id = __shfl_sync(kAll, id, sub);
+                if (lane >> 3 == t) {
+                    my_id = id;
+                    filled = n;
+                }
+            }
+        }
+    }
+    float w = 0.0f;
+    if (sub < filled) {
+        const float logit = route_logit(p, token, static_cast<uint32_t>(my_id));
+        w = p.softmax ? route_exp_diff(logit, max) * inv_total : __fdividef(1.0f, 1.0f + expf(-logit));
+    }
+    if (p.renormalize) {
+        float sum = w;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) {
+            sum += __shfl_xor_sync(kAll, sum, off);
+        }
+        w = sum > 0.0f ? __fdiv_rn(w, sum) : 0.0f;
+    }
+    w *= p.scaling;
+    if (sub < p.top_k && token < p.tokens) {
+        const uint64_t at = static_cast<uint64_t>(token) * p.top_k + sub;
+        p.ids[at] = sub < filled ? my_id : -1;
+        p.weights[at] = sub < filled ? w : 0.0f;
     }
 }
 

@@ -65,6 +65,37 @@ def test_route_many_tokens(cuda):
                                None if bb is None else bb.double().cpu().numpy(), 8, 4, True, True))
 
 
+@pytest.mark.parametrize("e,k,groups,kept", [(17, 8, 1, 1), (60, 4, 1, 1), (64, 8, 8, 3), (64, 1, 4, 2), (96, 6, 3, 1),
+                                             (128, 8, 8, 8), (128, 7, 4, 2), (200, 5, 1, 1), (256, 8, 4, 2), (256, 8, 8, 1)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_route_batches_with_holes_and_ties(cuda, e, k, groups, kept, dtype):
+    """Batches that share warps among tokens: coarse logits (many equal), masked ones, whole rows and groups of them, and
+    biases that bring different logits to within 1e-7 of one another."""
+    import torch
+    from catlass_b200 import capi
+    t = 4103
+    rng = np.random.default_rng(e + k)
+    x = (1.5 * rng.standard_normal((t, e))).astype(np.float32)
+    x[::3] = np.round(x[::3] * 4) / 4
+    x[1::7][rng.random((len(x[1::7]), e)) < 0.7] = -np.inf
+    x[5::11, : e // groups] = np.nan
+    x[40] = -np.inf
+    x[41, 1:] = -np.inf
+    logits = torch.from_numpy(x).to(cuda).to(getattr(torch, dtype))
+    x = logits.double().cpu().numpy()
+    with np.errstate(over="ignore"):
+        s = 1 / (1 + np.exp(-np.nan_to_num(x[0], nan=0.0)))
+    biases = [None, np.zeros(e, np.float32), (0.1 * rng.standard_normal(e)).astype(np.float32), (0.9 - s).astype(np.float32)]
+    for sigmoid in (True, False):
+        for bias in biases:
+            for top2 in (True, False):
+                w, ids = call(torch, capi, logits, k, bias=None if bias is None else torch.from_numpy(bias).to(cuda),
+                              groups=groups, groups_kept=kept, renormalize=top2,
+                              score=capi.ROUTE_SIGMOID if sigmoid else capi.ROUTE_SOFTMAX,
+                              group_score=capi.ROUTE_GROUP_TOP2_SUM if top2 else capi.ROUTE_GROUP_MAX)
+                check(w, ids, *R.route(x, k, sigmoid, bias, groups, kept, top2, top2))
+
+
 def test_route_ties_and_near_ties(cuda):
     import torch
     from catlass_b200 import capi
