@@ -25,13 +25,39 @@ struct NvPlan {
     bool pack_a, pack_b;
     uint32_t tile_rows;      // rows per row tile: 128 (few) or 256
     uint32_t max_tiles;      // row tiles at most
+    uint32_t sfa_blocks;     // 128-row scale blocks of A: a row tile's own, or those of all rows of a dense problem
     uint32_t words, sfb_blocks, matrices;
     uint64_t table_bytes, sfa_bytes, sfb_bytes;
     uint64_t total() const { return table_bytes + sfa_bytes + sfb_bytes; }
 };
 
-// The kernel for a problem.  The pair kernel's tile is 256 x 256 on two SMs, the few kernel's 128 weight rows x up to 128
-// rows of A on one: a row tile that is mostly padding, or too few tiles to fill the SMs, is cheaper on the latter.
+uint32_t nv_few_rows(const NvProblem& q)  // rows of A a stage has room for
+{
+    uint32_t mt = 16;
+    while (mt < q.m && mt < 128u) {
+        mt *= 2;
+    }
+    return mt;
+}
+
+// CTAs of a cluster along K: as many as leave every cluster at most one item and every CTA two stages, with partial sums
+// of 64 KB at most.
+uint32_t nv_few_splits(uint32_t mt, uint64_t items, uint32_t stages, uint32_t ctas)
+{
+    uint32_t splits = 1;
+    while (splits < 8u && items * splits * 2u <= ctas && stages >= 4u * splits &&
+           nv_few_partial_bytes(mt, splits * 2u) <= 64u * 1024u) {
+        splits *= 2;
+    }
+    return splits;
+}
+
+// Which kernel.  nvfp4_few_kernel reads weights a little faster (128-row tiles, deeper ring) and can split K, but every
+// row of A costs it more.  Measured, few / pair, us.  Grouped, rows per group on average (64 groups, n 4096, k 7168):
+// 4: 186 / 195, 16: 188 / 200, 32: 199 / 203, 64: 244 / 209; (128 groups, n 1024, k 2048): 16: 39 / 49, 64: 51 / 51.
+// Dense, m x n x k: 16 x 14336 x 4096: 11.3 / 12.7, 64 x: 13.3 / 12.6; 16 x 4096 x 14336: 12.4 / 24.5; 32 x 1024 x 2048: 6.4
+// / 7.1, 64 x: 8.3 / 7.5.  For dense problems the model below is fitted to those: a row of A costs the few kernel 60 ns, a
+// stage either kernel 0.3 us in each of its waves, the pair kernel 2 us more per call.
 bool nv_use_few(const NvProblem& q)
 {
     const long v = dev_knob("CB200_NV_FEW", -1);
@@ -39,9 +65,18 @@ bool nv_use_few(const NvProblem& q)
         return v != 0;
     }
     if (q.group_count != 0) {
-        return q.m / q.group_count <= 64u;
+        return q.m / q.group_count <= 32u;
     }
-    return q.m <= 128u;
+    if (q.m > 128u) {
+        return false;
+    }
+    constexpr uint64_t kSms = 148;
+    const uint32_t stages = (q.k + kNvStageK - 1u) / kNvStageK;
+    const uint64_t items = (q.n + 127u) / 128u, tiles = (q.n + kNvTileW - 1u) / kNvTileW;
+    const uint64_t splits = nv_few_splits(nv_few_rows(q), items, stages, kSms);
+    const uint64_t few = 60ull * q.m + 300ull * ((stages + splits - 1) / splits) * ((items * splits + kSms - 1) / kSms);
+    const uint64_t pair = 2000ull + 300ull * stages * ((tiles + kSms / 2 - 1) / (kSms / 2));
+    return few <= pair;
 }
 
 int plan_nv(const NvProblem& q, NvPlan* plan)
@@ -86,8 +121,8 @@ int plan_nv(const NvProblem& q, NvPlan* plan)
     plan->pack_a = q.group_count != 0 || q.scale_a_layout == CB200_NVFP4_SCALES_ROWS;
     plan->pack_b = q.scale_b_layout == CB200_NVFP4_SCALES_ROWS;
     plan->table_bytes = q.group_count == 0 ? 0 : align256(static_cast<uint64_t>(plan->max_tiles) * 16u + 16u);
-    plan->sfa_bytes =
-        plan->pack_a ? static_cast<uint64_t>(plan->max_tiles) * (plan->tile_rows / 128u) * plan->words * 512u : 0;
+    plan->sfa_blocks = q.group_count != 0 ? plan->max_tiles * (plan->tile_rows / 128u) : (q.m + 127u) / 128u;
+    plan->sfa_bytes = plan->pack_a ? static_cast<uint64_t>(plan->sfa_blocks) * plan->words * 512u : 0;
     plan->sfb_bytes = plan->pack_b ? static_cast<uint64_t>(plan->sfb_blocks) * plan->matrices * plan->words * 512u : 0;
     return CB200_SUCCESS;
 }
@@ -143,8 +178,7 @@ int launch_nv_pair(const NvProblem& q, const NvPlan& plan, NvParams p, const Dev
              : encode_nv_scales(&tmap_sfw, p.sfb, plan.words, static_cast<uint64_t>(plan.sfb_blocks) * plan.matrices);
     rc = rc != CB200_SUCCESS
              ? rc
-             : encode_nv_scales(&tmap_sfx, p.sfa, plan.words,
-                                plan.pack_a ? static_cast<uint64_t>(plan.max_tiles) * 2u : (q.m + 127u) / 128u);
+             : encode_nv_scales(&tmap_sfx, p.sfa, plan.words, plan.sfa_blocks);
     // rows of D that do not start on 16-byte boundaries are stored by the threads
     p.tma_store = (q.n * float_bytes(q.d_type)) % 16u == 0 ? 1u : 0u;
     CUtensorMap tmap_d = tmap_w;
@@ -184,10 +218,7 @@ int launch_nv_few(const NvProblem& q, const NvPlan& plan, const NvParams& p, con
 {
     NvFewParams fp;
     fp.g = p;
-    fp.mt = 16;
-    while (fp.mt < q.m && fp.mt < 128u) {
-        fp.mt *= 2;
-    }
+    fp.mt = nv_few_rows(q);
     CUtensorMap tmap_w, tmap_x;
     int rc = encode_nv_weights(&tmap_w, q, plan);
     rc = rc != CB200_SUCCESS ? rc : encode_nv_rows(&tmap_x, q, 16);
@@ -212,14 +243,8 @@ int launch_nv_few(const NvProblem& q, const NvPlan& plan, const NvParams& p, con
     if (q.block_num != 0 && q.block_num < ctas) {
         ctas = q.block_num;
     }
-    // K is split while every cluster still gets one item at most, every CTA at least two stages and the partial sums
-    // stay small
     const uint64_t items = static_cast<uint64_t>(plan.max_tiles) * plan.sfb_blocks;
-    fp.splits = 1;
-    while (fp.splits < 8u && items * fp.splits * 2u <= ctas && p.num_k_blocks >= 4u * fp.splits &&
-           nv_few_partial_bytes(fp.mt, fp.splits * 2u) <= 64u * 1024u) {
-        fp.splits *= 2;
-    }
+    fp.splits = nv_few_splits(fp.mt, items, p.num_k_blocks, ctas);
     fp.stages = kNvFewMaxStages;
     while (nv_few_smem_bytes(fp.mt, fp.stages, fp.splits) > kNvFewSmemBudget) {
         --fp.stages;
@@ -296,7 +321,7 @@ int run_nv(const NvProblem& q, void* stream_v)
             a.table = table;
             a.num_row_tiles = num_tiles;
         }
-        const uint64_t items = static_cast<uint64_t>(plan.max_tiles) * plan.tile_rows * ((plan.words + 3u) / 4u);
+        const uint64_t items = static_cast<uint64_t>(plan.sfa_blocks) * 128u * ((plan.words + 3u) / 4u);
         const uint64_t want = (items + kNvPackThreads - 1) / kNvPackThreads;
         const uint64_t cap = static_cast<uint64_t>(dev->sm_count) * 4u;
         nvfp4_pack_scales_kernel<<<static_cast<uint32_t>(want < cap ? want : cap), kNvPackThreads, 0, stream>>>(a);

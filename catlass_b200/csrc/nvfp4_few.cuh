@@ -6,15 +6,16 @@
 // (9/16 byte per weight).  With few items the K range of an item is split over the CTAs of a cluster: their fp32
 // partial sums go to the first CTA's shared memory and are added in rank order, the same bits on every run.
 //   warp 0  producer: weights and rows of A (tensor maps), both scale blocks (bulk copies)
-//   warp 1  MMA issuer        warps 2, 3  scale copiers (weights, rows of A): smem -> TMEM
-//   warps 4-7  epilogue, under the next item's MMAs (two accumulators)
+//   warp 1  MMA issuer        warps 2-5  scale copiers, one per word of a stage: smem -> TMEM
+//   warps 6-9  epilogue, under the next item's MMAs (two accumulators)
 #pragma once
 
 #include "nvfp4_gemm.cuh"
 
 namespace cb200 {
 
-constexpr int kNvFewThreads = 256;
+constexpr int kNvFewThreads = 320;
+constexpr uint32_t kNvFewCopiers = 4;
 constexpr int kNvFewEpiThreads = 128;
 constexpr int kNvFewMaxStages = 8;
 constexpr uint32_t kNvFewWBytes = 128 * kBlockKBytes;              // 16 KB of weights per stage
@@ -83,7 +84,7 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         for (uint32_t s = 0; s < fp.stages; ++s) {
             mbar_init(bar_full + s * 8, 1);
             mbar_init(bar_empty + s * 8, 1);
-            mbar_init(bar_sf_full + s * 8, 2);
+            mbar_init(bar_sf_full + s * 8, kNvFewCopiers);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(bar_tmem_full + a * 8, 1);
@@ -217,10 +218,11 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             }
         }
         __syncwarp();
-    } else if (warp < 4) {
-        // copier 2: the weights' scales to columns [0, 16) of the stage's slot; copier 3: those of A to [16, 32)
+    } else if (warp < 2 + kNvFewCopiers) {
+        // Copier w moves word w of the weights' scales to columns [4w, 4w + 4) of the stage's slot and that of A's to 16
+        // columns behind.  (A stage's last words may be missing: then there is nothing to move, the arrival stays.)
         if (lane == 0) {
-            const uint32_t which = warp - 2;
+            const uint32_t w = warp - 2;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = first_item; ok && idx < items; idx += item_step) {
@@ -230,11 +232,11 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t ssf = ring + stage * stage_bytes + kNvFewWBytes + which * 2048;
-                    const uint32_t slot = tmem_base + kSfBase + stage * kSfSlot + which * 16;
-                    const uint32_t words = words_of(kb);
-                    for (uint32_t w = 0; w < words; ++w) {
-                        tmem_cp_32x128b_warpx4(slot + w * 4, make_smem_desc_noswizzle(ssf + w * 512, 16, 128));
+                    const uint32_t ssf = ring + stage * stage_bytes + kNvFewWBytes + w * 512;
+                    const uint32_t slot = tmem_base + kSfBase + stage * kSfSlot + w * 4;
+                    if (w < words_of(kb)) {
+                        tmem_cp_32x128b_warpx4(slot, make_smem_desc_noswizzle(ssf, 16, 128));
+                        tmem_cp_32x128b_warpx4(slot + 16, make_smem_desc_noswizzle(ssf + 2048, 16, 128));
                     }
                     umma_commit<1>(bar_sf_full + stage * 8);
                     if (++stage == fp.stages) {
@@ -298,23 +300,14 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
                     uint32_t r[16];
                     tmem_ld_32x32b_x16(taddr + c * 16, r);
                     tmem_ld_wait();
+                    for (uint32_t s = 1; s < fp.splits; ++s) {  // (sixteen reads of a peer's sums in flight)
+                        const float* sums_of = s_partials + ((s - 1) * fp.mt + c * 16) * 128 + lane_row;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint32_t token = c * 16 + i;
-                        float v = __uint_as_float(r[i]);
-                        for (uint32_t s = 1; s < fp.splits; ++s) {
-                            v += s_partials[((s - 1) * fp.mt + token) * 128 + lane_row];
-                        }
-                        v *= alpha;
-                        if (token < rows && col < p.n) {
-                            const uint64_t at = (static_cast<uint64_t>(it.row0) + token) * p.n + col;
-                            if (p.d_type == 0) {
-                                static_cast<float*>(p.d)[at] = v;
-                            } else {
-                                static_cast<uint16_t*>(p.d)[at] = pack_out1(v, p.d_type == 2);
-                            }
+                        for (int i = 0; i < 16; ++i) {
+                            r[i] = __float_as_uint(__uint_as_float(r[i]) + sums_of[i * 128]);
                         }
                     }
+                    nv_store_columns<16>(p, r, static_cast<uint32_t>(it.row0) + c * 16, rows - c * 16, col, alpha);
                 }
             }
             tcgen05_fence_before();
