@@ -10,7 +10,7 @@
 
 namespace cb200 {
 
-constexpr int kCombineThreads = 256;
+constexpr int kCombineThreads = 128;
 constexpr int kCombineMaxTopK = 32;
 
 struct CombineParams {
