@@ -52,12 +52,12 @@ uint32_t nv_few_splits(uint32_t mt, uint64_t items, uint32_t stages, uint32_t ct
     return splits;
 }
 
-// Which kernel.  nvfp4_few_kernel reads weights a little faster (128-row tiles, deeper ring) and can split K, but every
-// row of A costs it more.  Measured, few / pair, us.  Grouped, rows per group on average (64 groups, n 4096, k 7168):
-// 4: 186 / 195, 16: 188 / 200, 32: 199 / 203, 64: 244 / 209; (128 groups, n 1024, k 2048): 16: 39 / 49, 64: 51 / 51.
-// Dense, m x n x k: 16 x 14336 x 4096: 11.3 / 12.7, 64 x: 13.3 / 12.6; 16 x 4096 x 14336: 12.4 / 24.5; 32 x 1024 x 2048: 6.4
-// / 7.1, 64 x: 8.3 / 7.5.  For dense problems the model below is fitted to those: a row of A costs the few kernel 60 ns, a
-// stage either kernel 0.3 us in each of its waves, the pair kernel 2 us more per call.
+// Which kernel.  nvfp4_few_kernel reads weights faster (128-row tiles, a deeper ring) and can split K, but every row of A
+// costs it more.  Measured, few / pair, us.  Grouped, rows per group on average (64 groups, n 4096, k 7168): 4: 163 / 182, 32:
+// 174 / 191, 64: 185 / 197, 128: 241 / 223; (128 groups, n 1024, k 2048): 16: 35 / 45, 64: 42 / 48, 256: 88 / 71.
+// Dense, m x n x k: 16 x 14336 x 4096: 9.5 / 12.1, 128 x: 13.2 / 12.8; 16 x 4096 x 4096: 6.2 / 8.2, 128 x: 11.6 / 8.9; 16 x 4096 x
+// 14336: 10.8 / 21.0, 128 x: 20.5 / 22.4.  The model below is fitted to those (ns): a call, the rows of A, and the stages of
+// the longest CTA or the weights' way from memory.
 bool nv_use_few(const NvProblem& q)
 {
     const long v = dev_knob("CB200_NV_FEW", -1);
@@ -65,7 +65,7 @@ bool nv_use_few(const NvProblem& q)
         return v != 0;
     }
     if (q.group_count != 0) {
-        return q.m / q.group_count <= 32u;
+        return q.m / q.group_count <= 64u;
     }
     if (q.m > 128u) {
         return false;
@@ -74,8 +74,12 @@ bool nv_use_few(const NvProblem& q)
     const uint32_t stages = (q.k + kNvStageK - 1u) / kNvStageK;
     const uint64_t items = (q.n + 127u) / 128u, tiles = (q.n + kNvTileW - 1u) / kNvTileW;
     const uint64_t splits = nv_few_splits(nv_few_rows(q), items, stages, kSms);
-    const uint64_t few = 60ull * q.m + 300ull * ((stages + splits - 1) / splits) * ((items * splits + kSms - 1) / kSms);
-    const uint64_t pair = 2000ull + 300ull * stages * ((tiles + kSms / 2 - 1) / (kSms / 2));
+    const uint64_t weights = static_cast<uint64_t>(q.n) * q.k * 9u / 16u;  // bytes
+    const uint64_t few_stages = 330ull * ((stages + splits - 1) / splits) * ((items * splits + kSms - 1) / kSms);
+    const uint64_t pair_stages = 290ull * stages * ((tiles + kSms / 2 - 1) / (kSms / 2));
+    const uint64_t few_bytes = weights / 5500u, pair_bytes = weights / 4200u;
+    const uint64_t few = 3800ull + 45ull * q.m + (few_stages > few_bytes ? few_stages : few_bytes);
+    const uint64_t pair = 4000ull + 10ull * q.m + (pair_stages > pair_bytes ? pair_stages : pair_bytes);
     return few <= pair;
 }
 
@@ -115,7 +119,7 @@ int plan_nv(const NvProblem& q, NvPlan* plan)
     plan->words = (q.k + 63u) / 64u;
     plan->sfb_blocks = (q.n + 127u) / 128u;
     if (static_cast<uint64_t>(plan->sfb_blocks) * plan->matrices > 0x7fffffffu ||
-        static_cast<uint64_t>(plan->max_tiles) * plan->sfb_blocks > 0x7fffffffu) {
+        static_cast<uint64_t>(plan->max_tiles) * 2u * plan->sfb_blocks > 0x7fffffffu) {
         return CB200_INVALID;  // tile and block numbers are 32-bit
     }
     plan->pack_a = q.group_count != 0 || q.scale_a_layout == CB200_NVFP4_SCALES_ROWS;
@@ -165,6 +169,29 @@ int encode_nv_output(CUtensorMap* map, const NvProblem& q)
     return encode_tmap_u8(map, q.d, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Rows of A per tile of a dense problem: the height whose waves over the pairs cost least.  (The scale blocks hold 128 rows:
+// 192-row tiles start at a block's beginning or middle.)
+uint32_t nv_tile_rows(uint32_t m, uint32_t n_tiles, uint32_t pairs)
+{
+    const long v = dev_knob("CB200_NV_TILEX", 0);
+    if (v != 0) {
+        return static_cast<uint32_t>(v);
+    }
+    constexpr uint32_t kRows[3] = {256, 192, 128};
+    constexpr uint64_t kCost[3] = {100, 80, 65};  // of a stage
+    uint32_t best = 0;
+    uint64_t best_cost = ~0ull;
+    for (uint32_t i = 0; i < 3; ++i) {
+        const uint64_t tiles = static_cast<uint64_t>((m + kRows[i] - 1u) / kRows[i]) * n_tiles;
+        const uint64_t cost = (tiles + pairs - 1u) / pairs * kCost[i];
+        if (cost < best_cost) {
+            best = kRows[i];
+            best_cost = cost;
+        }
+    }
+    return best;
+}
+
 int launch_nv_pair(const NvProblem& q, const NvPlan& plan, NvParams p, const DeviceState& dev, cudaStream_t stream)
 {
     CUtensorMap tmap_w, tmap_sfw, tmap_sfx;
@@ -206,7 +233,10 @@ int launch_nv_pair(const NvProblem& q, const NvPlan& plan, NvParams p, const Dev
     if (q.block_num != 0 && q.block_num / 2u < pairs) {
         pairs = q.block_num < 2u ? 1u : q.block_num / 2u;
     }
-    const uint64_t tiles = static_cast<uint64_t>(plan.max_tiles) * ((q.n + kNvTileW - 1u) / kNvTileW);
+    const uint32_t n_tiles = (q.n + kNvTileW - 1u) / kNvTileW;
+    p.tile_x = q.group_count != 0 ? kNvTileX : nv_tile_rows(q.m, n_tiles, pairs);
+    const uint64_t tiles =
+        static_cast<uint64_t>(q.group_count != 0 ? plan.max_tiles : (q.m + p.tile_x - 1u) / p.tile_x) * n_tiles;
     pairs = tiles < pairs ? static_cast<uint32_t>(tiles) : pairs;
     CB200_CUDA_TRY(launch_dependent(nvfp4_pair_kernel, 2 * pairs, kNvPairThreads, NvPairSmem::kTotalBytes, stream,
                                     tmap_w, tmap_x, tmap_sfw, tmap_sfx, tmap_d, p));
@@ -350,6 +380,7 @@ int run_nv(const NvProblem& q, void* stream_v)
     p.table = q.group_count != 0 ? table : nullptr;
     p.num_row_tiles = q.group_count != 0 ? num_tiles : nullptr;
     p.tma_store = 0;
+    p.tile_x = kNvTileX;
     return plan.few ? launch_nv_few(q, plan, p, *dev, stream) : launch_nv_pair(q, plan, p, *dev, stream);
 }
 

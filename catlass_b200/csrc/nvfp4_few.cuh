@@ -141,7 +141,7 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     auto words_of = [&](uint32_t kb) { return p.words - kb * 4 < 4 ? p.words - kb * 4 : 4u; };
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = first_item; ok && idx < items; idx += item_step) {
@@ -176,7 +176,7 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
             for (uint32_t idx = first_item; ok && idx < items; idx += item_step) {
@@ -221,7 +221,7 @@ nvfp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     } else if (warp < 2 + kNvFewCopiers) {
         // Copier w moves word w of the weights' scales to columns [4w, 4w + 4) of the stage's slot and that of A's to 16
         // columns behind.  (A stage's last words may be missing: then there is nothing to move, the arrival stays.)
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t w = warp - 2;
             uint32_t stage = 0, phase = 0;
             bool ok = true;

@@ -35,6 +35,7 @@ struct NvParams {
     const int4* table;             // grouped: [row tile] = (first row, one past the group's last row, group, 0)
     const uint32_t* num_row_tiles; // grouped: entries of the table
     uint32_t tma_store;            // pair kernel: D has a tensor map
+    uint32_t tile_x;               // pair kernel, dense: rows of A per tile, 128, 192 or 256
 };
 
 // Instruction descriptor of kind::mxf4nvf4 with E4M3 scales (bit 23 = 0); with 16-element blocks an MMA uses all four
@@ -229,6 +230,10 @@ nvfp4_pack_scales_kernel(const NvPackParams p)
 // rows then cost what they are: an MMA of N columns takes N/256 of a full one and reads N/256 of A, where rows of A on the
 // M axis would be padded to 256.  And a warp that stores a row of D writes 32 neighbouring columns.
 //
+// The single threads of the pipeline are picked by elect.sync: the compiler then knows that one thread runs their loops and
+// keeps what tcgen05 and TMA instructions take in uniform registers.  With lane == 0 instead, issuing them set the pace of
+// small tiles (128 x 4096 x 4096: 10.7 us against 8.7).
+//
 // Per stage (256 along K) a CTA takes in its weights 16 KB, half of the tile's rows of A (up to 16 KB) and the scale blocks
 // of its weight rows (2 KB) and of all rows of A (2 x 2 KB), and the tensor core reads 16 + 16 + 6 KB of it: 76 KB through
 // a shared memory of 128 bytes a clock are 608 clocks, against 512 of MMAs.  Measured with a full tile: 714 a stage.
@@ -386,7 +391,7 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     grid_launch_dependents();
     grid_dependency_wait();  // the packed scales, the table and the operands of the kernels before
 
-    const uint32_t m_tiles = grouped ? *p.num_row_tiles : (p.m + kNvTileX - 1) / kNvTileX;
+    const uint32_t m_tiles = grouped ? *p.num_row_tiles : (p.m + p.tile_x - 1) / p.tile_x;
     const uint32_t n_tiles = (p.n + kNvTileW - 1) / kNvTileW;
     const uint32_t total_tiles = m_tiles * n_tiles;
     const uint32_t num_kb = p.num_k_blocks;
@@ -395,6 +400,8 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         uint32_t row0;      // first row of A
         uint32_t rows;      // rows of A to store, 1 .. 256
         uint32_t cols;      // ... padded to a multiple of 32: columns of the MMA
+        uint32_t block_x;   // the scale block of the first row, and the row's place in it (0, or 64 with 192-row tiles)
+        uint32_t shift;
         uint32_t group;
     };
     auto get = [&](uint32_t idx) {
@@ -406,19 +413,24 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             t.row0 = static_cast<uint32_t>(e.x);
             end = static_cast<uint32_t>(e.y);
             t.group = static_cast<uint32_t>(e.z);
+            t.block_x = 2 * t.mt;
+            t.shift = 0;
         } else {
-            t.row0 = t.mt * kNvTileX;
+            t.row0 = t.mt * p.tile_x;
             end = p.m;
             t.group = 0;
+            t.block_x = t.row0 / 128;
+            t.shift = t.row0 % 128;
         }
-        t.rows = end - t.row0 < kNvTileX ? end - t.row0 : kNvTileX;
+        const uint32_t most = grouped ? kNvTileX : p.tile_x;
+        t.rows = end - t.row0 < most ? end - t.row0 : most;
         t.cols = (t.rows + 31u) & ~31u;
         return t;
     };
 
     if (warp == 0) {
         // ---------------------------------------------------------------- operand producer (both CTAs)
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
@@ -428,7 +440,7 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 const uint32_t x_bytes = (16u << which) * kBlockKBytes;
                 const uint32_t x0 = t.row0 + cta_rank * half;
                 const uint32_t w0 = t.nt * kNvTileW + cta_rank * 128;
-                const uint32_t sf_x = t.cols > 128 ? 4096u : 2048u;
+                const uint32_t sf_x = t.shift + t.cols > 128 ? 4096u : 2048u;
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_empty + stage * 8, phase ^ 1, s_abort, p.status, kDevTimeoutProducer);
                     if (!ok) {
@@ -453,13 +465,13 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         __syncwarp();
     } else if (warp == 2) {
         // ---------------------------------------------------------------- scale producer (both CTAs)
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
                 const Tile t = get(idx);
                 const int32_t block_w = static_cast<int32_t>(t.group * p.sfb_blocks + 2 * t.nt + cta_rank);
-                const int32_t block_x = static_cast<int32_t>(2 * t.mt);
+                const int32_t block_x = static_cast<int32_t>(t.block_x);
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_empty + stage * 8, phase ^ 1, s_abort, p.status, kDevTimeoutProducer);
                     if (!ok) {
@@ -472,7 +484,7 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                     // and columns are not stored)
                     tma_load_3d_pair(ssf, &tmap_sfw, full, 0, w2, block_w);
                     tma_load_3d_pair(ssf + 2048, &tmap_sfx, full, 0, w2, block_x);
-                    if (t.cols > 128) {
+                    if (t.shift + t.cols > 128) {
                         tma_load_3d_pair(ssf + 4096, &tmap_sfx, full, 0, w2, block_x + 1);
                     }
                     if (++stage == kStages) {
@@ -485,11 +497,13 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (leader CTA only)
-        if (lane == 0 && cta_rank == 0) {
+        if (cta_rank == 0 && elect_one()) {
             uint32_t stage = 0, phase = 0, acc_phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
-                const uint32_t idesc = make_idesc_nv(kNvTileW, get(idx).cols);
+                const Tile t = get(idx);
+                const uint32_t idesc = make_idesc_nv(kNvTileW, t.cols);
+                const uint32_t skip = t.shift / 32;  // scale columns of rows in front of the tile
                 ok = mbar_wait(bar_tmem_empty, acc_phase ^ 1, s_abort, p.status, kDevTimeoutMmaTmem);
                 if (!ok) {
                     break;
@@ -505,7 +519,7 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                     const uint32_t sw = ring + stage * S::kStageBytes;
                     const uint32_t sx = sw + S::kWBytes;
                     const uint32_t t_sfw = tmem_base + kAccCols + stage * kSfSlot;
-                    const uint32_t t_sfx = t_sfw + 16;
+                    const uint32_t t_sfx = t_sfw + 16 + skip;
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         const uint64_t dw = make_smem_desc_sw128(sw + j * 32, 16, 1024);
@@ -531,11 +545,12 @@ nvfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         // Copier w moves word w of the scale blocks.  Slot `stage` is free when the stage's "full" barrier fires: the
         // MMAs that read it completed before the producers were allowed to refill the stage.
         const uint32_t w = warp - 3;
-        if (lane == 0 && cta_rank == 0) {
+        if (cta_rank == 0 && elect_one()) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t idx = pair; ok && idx < total_tiles; idx += num_pairs) {
-                const bool two = get(idx).cols > 128;
+                const Tile t = get(idx);
+                const bool two = t.shift + t.cols > 128;
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = mbar_wait(bar_full + stage * 8, phase, s_abort, p.status, kDevTimeoutConvert);
                     if (!ok) {

@@ -67,7 +67,8 @@ def test_matmul_matches_the_product(cuda, m, n, k, dtype):
             assert close(d.double().cpu().numpy(), want, size, k, dtype), (la, lb)
 
 
-@pytest.mark.parametrize("m,n,k,block_num", [(16, 512, 2048, 4), (200, 512, 512, 1), (600, 600, 320, 5), (64, 4096, 1024, 0)])
+@pytest.mark.parametrize("m,n,k,block_num", [(16, 512, 2048, 4), (200, 512, 512, 1), (600, 600, 320, 5), (64, 4096, 1024, 0),
+                                             (700, 200, 352, 8), (768, 256, 1056, 8)])  # (four tiles of 192 rows)
 def test_matmul_without_alpha_on_few_ctas(cuda, m, n, k, block_num):
     import torch
     from catlass_b200 import capi
