@@ -351,8 +351,8 @@ int run_nv(const NvProblem& q, void* stream_v)
             a.table = table;
             a.num_row_tiles = num_tiles;
         }
-        const uint64_t items = static_cast<uint64_t>(plan.sfa_blocks) * 128u * ((plan.words + 3u) / 4u);
-        const uint64_t want = (items + kNvPackThreads - 1) / kNvPackThreads;
+        const uint64_t warps = static_cast<uint64_t>(plan.sfa_blocks) * ((plan.words + 3u) / 4u);
+        const uint64_t want = (warps + kNvPackThreads / 32 - 1) / (kNvPackThreads / 32);
         const uint64_t cap = static_cast<uint64_t>(dev->sm_count) * 4u;
         nvfp4_pack_scales_kernel<<<static_cast<uint32_t>(want < cap ? want : cap), kNvPackThreads, 0, stream>>>(a);
         CB200_CUDA_TRY(cudaGetLastError());

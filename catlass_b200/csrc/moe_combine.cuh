@@ -1,5 +1,8 @@
 // Combine: out[t] = round( shared_weight * shared[t] + sum_j weights[t][j] * d[position[t][j]] ), fp32, j ascending.
-// HBM-bound: every row of D is read once, 16 bytes per thread and row, all rows of a token in flight together.
+// HBM-bound: every row of D is read once, 16 bytes per thread and row, eight rows of a token in flight together.
+// 8192 tokens x 8 rows x 7168 bf16: 169 us, 6.26 TB/s, 0.96 of the HBM copy rate (CTAs of 256 threads, whose last one of a
+// row is half empty: 179; of 64: 168, but 10.0 us instead of 6.5 for 7698 x 8 x 91 fp32).  Rows that do not start on 16-byte
+// boundaries are read element by element: 1024 x 8 x 4100 bf16: 40 us.
 #pragma once
 
 #include <cuda_bf16.h>

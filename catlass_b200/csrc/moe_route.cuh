@@ -7,6 +7,9 @@
 // One warp per token, kPer consecutive logits per lane, read once with wide loads; everything else happens in
 // registers, shuffles and redux.sync.  A lane sorts its keys, the warp picks the largest of the lanes' first keys.
 //
+// Bound by instruction issue and, for one token, by latency: ~950 instructions per token here, ~450 in the kernel that
+// shares a warp among four tokens (below); reading 16384 x 256 bf16 logits takes 1.4 us of the 16.4.
+//
 // Order.  The ids have to be those of the exact keys, but 32-bit scores carry a few units in the last place of error.
 // Keys are compared as order-preserving integers; the kernel knows how far a 32-bit key can be off, and when two
 // neighbours of the selected order are closer than that, the candidates' keys are worked out in 64 bits, a lane each.

@@ -5,6 +5,9 @@
 // wasted.  A persistent CTA walks (row tile, 128-column block) items; HBM-bound on the weights and their scales
 // (9/16 byte per weight).  With few items the K range of an item is split over the CTAs of a cluster: their fp32
 // partial sums go to the first CTA's shared memory and are added in rank order, the same bits on every run.
+// 256 rows of 64 experts, n 4096, k 7168: 154 - 163 us (weights 1.06 GB: the HBM copy rate); 16 x 14336 x 4096: 9.5 us; 16 x
+// 4096 x 14336, four CTAs per tile: 10.8.  Weights arrive as fast as HBM gives them; a call of its own costs ~4 us, a row of A
+// 45 ns.
 //   warp 0  producer: weights and rows of A (tensor maps), both scale blocks (bulk copies)
 //   warp 1  MMA issuer        warps 2-5  scale copiers, one per word of a stage: smem -> TMEM
 //   warps 6-9  epilogue, under the next item's MMAs (two accumulators)

@@ -3,7 +3,9 @@
 //   scale = e4m3( amax / (6 * tensor_scale) ),   q[i] = e2m1( x[i] * (1 / (scale * tensor_scale)) )
 //
 // A thread owns a block: it reads its 16 values with 16-byte loads, nothing is exchanged between threads.  HBM-bound:
-// 2 (or 4) bytes read and 9/16 of a byte written per element.
+// 2 (or 4) bytes read and 9/16 of a byte written per element.  bf16 32768 x 7168: 99 us = 6.1 TB/s (0.93 of the HBM copy
+// rate), scales tiled 102; fp32 8192 x 8192: 6.5 TB/s; SwiGLU in front, bf16 8192 x 4096: 27 us = 5.8 TB/s.  175 instructions
+// per block keep the SMs two thirds busy; without the next block's loads in flight the same took 126 us.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -637,7 +637,8 @@ CB200_API int cb200_moe_route(const cb200_moe_route_args *args, void *stream);
  * cb200_moe_combine read.  The outputs hold tokens * top_k rows; rows past the last expert's are left as they were.
  * Requirements: x, its rows (x_pitch) and q 16-byte aligned, k a multiple of 16 (INT8, NVFP4) or 32 (MX_E4M3), or of 16
  * bytes (COPY); tokens * top_k < 2^24.  The workspace (cb200_moe_dispatch_workspace_size bytes, 256-byte aligned)
- * holds counts.  The reference has no such kernel: its examples sort and quantise on the host.
+ * holds counts; calls that may run at the same time (other streams, other graphs) need one each.  The reference has no
+ * such kernel: its examples sort and quantise on the host.
  */
 #define CB200_DISPATCH_INDEX 0
 #define CB200_DISPATCH_COPY 1
@@ -752,7 +753,8 @@ CB200_API uint64_t cb200_nvfp4_tiled_scale_bytes(uint32_t rows, uint32_t k);
  * alpha: device scalar, the product of the two tensor scales, or NULL for 1.
  * Requirements: k a multiple of 32; a, b, the scales and the workspace 16-byte aligned (the workspace 256).
  * Scales that come by rows are re-tiled into the workspace first (cb200_nvfp4_matmul_workspace_size bytes, 0 when both
- * are tiled): one extra pass over them.  Keep the weights' scales tiled.
+ * are tiled): one extra pass over them.  Keep the weights' scales tiled.  Calls that may run at the same time need a
+ * workspace each.
  * The fp32 sums are those of the tensor core over K, in chunks of 64; few rows of A may split K over the CTAs of a
  * cluster, whose partial sums are added in a fixed order.  The same call gives the same bits on every run.
  */
