@@ -143,28 +143,26 @@ cudaError_t launch_rows_format(const DispatchParams& p, uint32_t format, uint32_
     }
 }
 
-template <int kDType, int kVec>
-cudaError_t launch_combine_out(const CombineParams& p, uint32_t out_type, const DeviceState& dev, cudaStream_t stream)
+template <int kDType, int kVec, int kCols, int kSlots>
+cudaError_t launch_combine_out(const CombineParams& p, uint32_t out_type, cudaStream_t stream)
 {
-    const uint32_t chunks = (p.n + kCombineThreads * kVec - 1) / (kCombineThreads * kVec);
-    (void)dev;
-    const dim3 grid(chunks, p.tokens < 65535u ? p.tokens : 65535u, 1);
+    constexpr uint32_t kWide = kCombineThreads * kVec * kCols;
+    const dim3 grid((p.n + kWide - 1) / kWide, p.tokens < 65535u ? p.tokens : 65535u, 1);
     switch (out_type) {
-        case CB200_DTYPE_F32: moe_combine_kernel<kDType, 0, kVec><<<grid, kCombineThreads, 0, stream>>>(p); break;
-        case CB200_DTYPE_BF16: moe_combine_kernel<kDType, 1, kVec><<<grid, kCombineThreads, 0, stream>>>(p); break;
-        default: moe_combine_kernel<kDType, 2, kVec><<<grid, kCombineThreads, 0, stream>>>(p); break;
+        case CB200_DTYPE_F32: moe_combine_kernel<kDType, 0, kVec, kCols, kSlots><<<grid, kCombineThreads, 0, stream>>>(p); break;
+        case CB200_DTYPE_BF16: moe_combine_kernel<kDType, 1, kVec, kCols, kSlots><<<grid, kCombineThreads, 0, stream>>>(p); break;
+        default: moe_combine_kernel<kDType, 2, kVec, kCols, kSlots><<<grid, kCombineThreads, 0, stream>>>(p); break;
     }
     return cudaGetLastError();
 }
 
-template <int kVec>
-cudaError_t launch_combine(const CombineParams& p, uint32_t d_type, uint32_t out_type, const DeviceState& dev,
-                           cudaStream_t stream)
+template <int kVec, int kCols, int kSlots>
+cudaError_t launch_combine(const CombineParams& p, uint32_t d_type, uint32_t out_type, cudaStream_t stream)
 {
     switch (d_type) {
-        case CB200_DTYPE_F32: return launch_combine_out<0, kVec>(p, out_type, dev, stream);
-        case CB200_DTYPE_BF16: return launch_combine_out<1, kVec>(p, out_type, dev, stream);
-        default: return launch_combine_out<2, kVec>(p, out_type, dev, stream);
+        case CB200_DTYPE_F32: return launch_combine_out<0, kVec, kCols, kSlots>(p, out_type, stream);
+        case CB200_DTYPE_BF16: return launch_combine_out<1, kVec, kCols, kSlots>(p, out_type, stream);
+        default: return launch_combine_out<2, kVec, kCols, kSlots>(p, out_type, stream);
     }
 }
 
@@ -399,10 +397,20 @@ int cb200_moe_combine(const cb200_moe_combine_args* a, void* stream_v)
     p.weights = a->weights;
     p.shared = a->shared;
     p.out = a->out;
-    // eight columns per thread where every row of every matrix starts on a 16-byte boundary
-    const bool vec = (a->n & 7u) == 0 && aligned16(a->d) && aligned16(a->out) && aligned16(a->shared);
-    CB200_CUDA_TRY(vec ? launch_combine<8>(p, a->d_type, a->out_type, *dev, stream)
-                       : launch_combine<1>(p, a->d_type, a->out_type, *dev, stream));
+    // eight columns per thread where every row of every matrix starts on a 16-byte boundary, else pairs where it starts
+    // on a pair's, else single ones, at four places each unless two CTAs cover a row
+    const uintptr_t all = reinterpret_cast<uintptr_t>(a->d) | reinterpret_cast<uintptr_t>(a->out) |
+                          reinterpret_cast<uintptr_t>(a->shared);
+    if ((a->n & 7u) == 0 && (all & 15u) == 0) {
+        CB200_CUDA_TRY((a->top_k <= 4u ? launch_combine<8, 1, 4>(p, a->d_type, a->out_type, stream)
+                                       : launch_combine<8, 1, 8>(p, a->d_type, a->out_type, stream)));
+    } else if ((a->n & 1u) == 0 && (all & 7u) == 0) {
+        CB200_CUDA_TRY((a->n <= 2u * 2u * kCombineThreads ? launch_combine<2, 1, 8>(p, a->d_type, a->out_type, stream)
+                                                          : launch_combine<2, 4, 8>(p, a->d_type, a->out_type, stream)));
+    } else {
+        CB200_CUDA_TRY((a->n <= 2u * kCombineThreads ? launch_combine<1, 1, 8>(p, a->d_type, a->out_type, stream)
+                                                     : launch_combine<1, 4, 8>(p, a->d_type, a->out_type, stream)));
+    }
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return CB200_SUCCESS;
 }
