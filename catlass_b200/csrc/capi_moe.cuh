@@ -471,7 +471,7 @@ int cb200_nvfp4_quantize(const cb200_nvfp4_quantize_args* a, void* stream_v)
     p.q = static_cast<uint8_t*>(a->q);
     p.scale = static_cast<uint8_t*>(a->scale);
     const uint64_t want = (static_cast<uint64_t>(p.rows) * p.blocks + kNvQuantThreads - 1) / kNvQuantThreads;
-    const uint64_t cap = static_cast<uint64_t>(dev->sm_count) * 8u;
+    const uint64_t cap = static_cast<uint64_t>(dev->sm_count) * nv_quant_ctas(a->x_type == CB200_DTYPE_F32 ? 0 : 1, swiglu);
     const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
     p.word_stores = p.blocks % 4u == 0 && aligned_to(a->scale, 4) ? 1u : 0u;
     p.step_rows = grid * kNvQuantThreads / p.blocks;

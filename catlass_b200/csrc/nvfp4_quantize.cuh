@@ -3,9 +3,9 @@
 //   scale = e4m3( amax / (6 * tensor_scale) ),   q[i] = e2m1( x[i] * (1 / (scale * tensor_scale)) )
 //
 // A thread owns a block: it reads its 16 values with 16-byte loads, nothing is exchanged between threads.  HBM-bound:
-// 2 (or 4) bytes read and 9/16 of a byte written per element.  bf16 32768 x 7168: 99 us = 6.1 TB/s (0.93 of the HBM copy
-// rate), scales tiled 102; fp32 8192 x 8192: 6.5 TB/s; SwiGLU in front, bf16 8192 x 4096: 27 us = 5.8 TB/s.  175 instructions
-// per block keep the SMs two thirds busy; without the next block's loads in flight the same took 126 us.
+// 2 (or 4) bytes read and 9/16 of a byte written per element.  bf16 32768 x 7168: 92 us = 6.5 TB/s, the HBM copy rate, scales
+// tiled 94; 4111 x 7168: 14 us; fp32 8192 x 8192: 6.6 TB/s; SwiGLU in front, bf16 8192 x 4096: 27 us = 5.7 TB/s.  180
+// instructions per block keep the SMs two thirds busy; without the next block's loads in flight the first took 126 us.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -18,6 +18,8 @@
 namespace cb200 {
 
 constexpr int kNvQuantThreads = 256;
+// CTAs of the quantiser that fit an SM; the grid is one such wave (more CTAs than that run in a second, emptier one)
+__host__ __device__ constexpr int nv_quant_ctas(int type, bool swiglu) { return type == 0 || swiglu ? 4 : 5; }
 
 // Eight values times inv -> eight E2M1 codes, value i in nibble i (nearest, ties to even, at most 6).
 __device__ __forceinline__ uint32_t e2m1_codes8(const float* v, float inv)
@@ -168,7 +170,7 @@ struct Raw16 {
 // The next block's loads are in flight while a block is worked on.  A thread's blocks are gridDim * 256 apart; (row, block) advance by that step without a division.  Four neighbouring
 // lanes hold the four bytes of a scale word where a row has whole words (p.word_stores): one of them stores it.
 template <int kType, bool kSwiglu>
-__global__ void __launch_bounds__(kNvQuantThreads)
+__global__ void __launch_bounds__(kNvQuantThreads, nv_quant_ctas(kType, kSwiglu))
 nvfp4_quantize_kernel(const NvQuantParams p)
 {
     grid_launch_dependents();

@@ -440,6 +440,96 @@ struct GroupedMxMatmulFinalizeRouting {
     static int Run(CArgs const* c, void* stream) { return cb200_mx_grouped_matmul_finalize_routing(c, stream); }
 };
 
+/// NVFP4 matmul (E2M1 with an E4M3 scale per 16 elements along K, D = alpha * A B): A row-major [m][k/2] bytes, B column-major
+/// [n][k/2] bytes.  The reference's 4-bit matmul is MXFP4 (MxMatmul above); the scale layouts are those of the C ABI.
+struct Nvfp4Matmul {
+    struct Arguments {
+        GemmCoord problemShape;
+        uint32_t aicCoreNum = 0;  // upper bound on CTAs (0 = one per SM)
+        uint8_t* ptrA = nullptr;
+        uint8_t* ptrB = nullptr;
+        uint8_t* ptrScaleA = nullptr;
+        uint8_t* ptrScaleB = nullptr;
+        float* ptrAlpha = nullptr;  // device scalar or null
+        uint8_t* ptrD = nullptr;
+        uint32_t scaleLayoutA = CB200_NVFP4_SCALES_ROWS;
+        uint32_t scaleLayoutB = CB200_NVFP4_SCALES_ROWS;
+        uint32_t dType = CB200_DTYPE_BF16;
+    };
+    using CArgs = cb200_nvfp4_matmul_args;
+    static CArgs ToUnderlyingArguments(Arguments const& a, void* workspace, size_t workspaceBytes)
+    {
+        CArgs c{};
+        c.m = a.problemShape.m();
+        c.n = a.problemShape.n();
+        c.k = a.problemShape.k();
+        c.scale_a_layout = a.scaleLayoutA;
+        c.scale_b_layout = a.scaleLayoutB;
+        c.d_type = a.dType;
+        c.a = a.ptrA;
+        c.b = a.ptrB;
+        c.scale_a = a.ptrScaleA;
+        c.scale_b = a.ptrScaleB;
+        c.alpha = a.ptrAlpha;
+        c.d = a.ptrD;
+        c.workspace = workspace;
+        c.workspace_bytes = workspaceBytes;
+        c.block_num = a.aicCoreNum;
+        return c;
+    }
+    static int CanImplement(CArgs const* c) { return cb200_nvfp4_matmul_can_implement(c); }
+    static uint64_t WorkspaceSize(CArgs const* c) { return cb200_nvfp4_matmul_workspace_size(c); }
+    static int Run(CArgs const* c, void* stream) { return cb200_nvfp4_matmul(c, stream); }
+};
+
+/// Grouped (slice-M) NVFP4 matmul: group g owns a run of rows of A and D, its own B, scales and alpha.
+template <class ElementGroupList = int64_t>
+struct GroupedNvfp4MatmulSliceM {
+    struct Arguments {
+        GemmCoord problemShape;
+        uint32_t problemCount = 0;
+        uint8_t* ptrGroupList = nullptr;
+        uint8_t* ptrA = nullptr;
+        uint8_t* ptrB = nullptr;
+        uint8_t* ptrScaleA = nullptr;  // by rows
+        uint8_t* ptrScaleB = nullptr;
+        float* ptrAlpha = nullptr;     // [problemCount] or null
+        uint8_t* ptrD = nullptr;
+        uint32_t scaleLayoutB = CB200_NVFP4_SCALES_ROWS;
+        uint32_t groupListKind = CB200_GROUP_LIST_SIZES;
+        uint32_t dType = CB200_DTYPE_BF16;
+        uint32_t aicCoreNum = 0;
+    };
+    using CArgs = cb200_nvfp4_grouped_matmul_args;
+    static CArgs ToUnderlyingArguments(Arguments const& a, void* workspace, size_t workspaceBytes)
+    {
+        static_assert(sizeof(ElementGroupList) == 8 || sizeof(ElementGroupList) == 4, "int64 or int32 group list");
+        CArgs c{};
+        c.m = a.problemShape.m();
+        c.n = a.problemShape.n();
+        c.k = a.problemShape.k();
+        c.group_count = a.problemCount;
+        c.scale_b_layout = a.scaleLayoutB;
+        c.group_list_type = sizeof(ElementGroupList) == 8 ? CB200_GROUP_LIST_INT64 : CB200_GROUP_LIST_INT32;
+        c.group_list_kind = a.groupListKind;
+        c.d_type = a.dType;
+        c.a = a.ptrA;
+        c.b = a.ptrB;
+        c.group_list = a.ptrGroupList;
+        c.scale_a = a.ptrScaleA;
+        c.scale_b = a.ptrScaleB;
+        c.alpha = a.ptrAlpha;
+        c.d = a.ptrD;
+        c.workspace = workspace;
+        c.workspace_bytes = workspaceBytes;
+        c.block_num = a.aicCoreNum;
+        return c;
+    }
+    static int CanImplement(CArgs const* c) { return cb200_nvfp4_grouped_matmul_slice_m_can_implement(c); }
+    static uint64_t WorkspaceSize(CArgs const* c) { return cb200_nvfp4_grouped_matmul_slice_m_workspace_size(c); }
+    static int Run(CArgs const* c, void* stream) { return cb200_nvfp4_grouped_matmul_slice_m(c, stream); }
+};
+
 }  // namespace Kernel
 
 namespace Device {

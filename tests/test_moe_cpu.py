@@ -143,6 +143,46 @@ def test_nvfp4_matmul_refusals(capi):
     assert capi.nvfp4_grouped_matmul_workspace_size(256, 4096, 7168, 64, 1) > 0
 
 
+CPP = r"""
+#include <cstdio>
+#include "catlass_b200/device_gemm.hpp"
+using namespace Catlass;
+int main() {
+    using Dense = Gemm::Device::DeviceGemm<Gemm::Kernel::Nvfp4Matmul>;
+    using Grouped = Gemm::Device::DeviceGemm<Gemm::Kernel::GroupedNvfp4MatmulSliceM<int32_t>>;
+    auto p = reinterpret_cast<uint8_t*>(256);
+    Gemm::Kernel::Nvfp4Matmul::Arguments a;
+    a.problemShape = GemmCoord{128, 256, 4096};
+    a.ptrA = a.ptrB = a.ptrScaleA = a.ptrScaleB = a.ptrD = p;
+    a.scaleLayoutB = CB200_NVFP4_SCALES_TILED;
+    Gemm::Kernel::GroupedNvfp4MatmulSliceM<int32_t>::Arguments g;
+    g.problemShape = GemmCoord{128, 256, 4096};
+    g.problemCount = 4;
+    g.ptrGroupList = g.ptrA = g.ptrB = g.ptrScaleA = g.ptrScaleB = g.ptrD = p;
+    bool ok = Dense::CanImplement(a) == Status::kSuccess && Grouped::CanImplement(g) == Status::kSuccess;
+    g.ptrGroupList = reinterpret_cast<uint8_t*>(260);   // aligned for int32, not for int64
+    ok = ok && Grouped::CanImplement(g) == Status::kSuccess;
+    size_t dense = Dense::GetWorkspaceSize(a);
+    a.problemShape = GemmCoord{128, 256, 40};
+    ok = ok && Dense::CanImplement(a) == Status::kInvalid;
+    std::printf("%d %zu\n", ok ? 1 : 0, dense);
+    return 0;
+}
+"""
+
+
+def test_cpp_descriptors(capi):
+    """The C++ descriptors of the NVFP4 matmuls compile, link and hand their members on."""
+    lib = capi.library_path()
+    with tempfile.TemporaryDirectory() as td:
+        src, exe = os.path.join(td, "t.cpp"), os.path.join(td, "t")
+        open(src, "w").write(CPP)
+        subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "include"), src, "-o", exe, lib,
+                        "-Wl,-rpath," + os.path.dirname(lib)], check=True)
+        out = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()
+    assert out == ["1", str(capi.nvfp4_tiled_scale_bytes(128, 4096))]
+
+
 def test_python_calls_check_their_tensors(capi):
     """Sizes and places of tensors are checked before an address is handed on."""
     torch = pytest.importorskip("torch")
