@@ -527,14 +527,27 @@ def _device(t, what):
     return t.get_device()
 
 
-def _buffer(t, nbytes, what, device):
-    """Address of a tensor of that device used as a raw buffer of at least `nbytes` bytes; None stays None."""
+def _sizes(bits, *values):
+    """Refuses sizes that the library's 32-bit fields would not hold as they are; bits: the values' bitwise or, which has
+    a sign or a bit from 31 up when one of them has."""
+    if bits >> 31:
+        raise ValueError(f"sizes must lie in [0, 2^31), got {values}")
+
+
+def _buffer(t, nbytes, what, device, itemsize=0):
+    """Address of a tensor of that device used as a raw buffer of at least `nbytes` bytes; None stays None.  With an
+    itemsize, a buffer of another size has to have elements of that many bytes (or one: raw bytes), which refuses a tensor
+    of the right shape and the wrong type."""
     if t is None:
         return None
     if t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous tensor of device {device}")
-    if t.nbytes < nbytes:
-        raise ValueError(f"{what} holds {t.nbytes} bytes, {nbytes} are needed")
+    have = t.nbytes
+    if have != nbytes:
+        if have < nbytes:
+            raise ValueError(f"{what} holds {have} bytes, {nbytes} are needed")
+        if itemsize and t.itemsize != itemsize and t.itemsize != 1:
+            raise ValueError(f"{what} must have elements of {itemsize} bytes, not {t.dtype}")
     return t.data_ptr()
 
 
@@ -542,13 +555,15 @@ def _rows(t, rows, width, pitch, elem, what, device):
     """As _buffer, for `rows` rows of `width` elements with `pitch` elements between them (a view with strided rows is
     taken: only the storage behind its first element has to be long enough)."""
     if not pitch:
-        return _buffer(t, rows * width * elem, what, device)
+        return _buffer(t, rows * width * elem, what, device, elem)
     if t is None:
         return None
     if t.get_device() != device:
         raise ValueError(f"{what} must be a tensor of device {device}")
+    if t.itemsize != elem and t.itemsize != 1:
+        raise ValueError(f"{what} must have elements of {elem} bytes, not {t.dtype}")
     need = ((rows - 1) * pitch + width) * elem if rows and width else 0
-    have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+    have = t.untyped_storage().nbytes() - t.storage_offset() * t.itemsize
     if have < need:
         raise ValueError(f"{what} holds {have} bytes, {need} are needed")
     return t.data_ptr()
@@ -578,13 +593,14 @@ def moe_route(logits, weights, ids, tokens, experts, top_k, score=ROUTE_SOFTMAX,
     """logits [tokens][experts] -> weights fp32 and ids int32 [tokens][top_k], the experts with the largest scores (plus
     bias) of the best groups, ties to the lower index; id -1 and weight 0 where no expert is left."""
     dev = _device(logits, "logits")
+    _sizes(tokens | experts | top_k | groups | logits_pitch, tokens, experts, top_k, groups, logits_pitch)
     out = tokens * top_k * 4
     args = MoeRouteArgs(tokens, experts, top_k, score, groups, groups if groups_kept is None else groups_kept,
                         group_score, ROUTE_RENORMALIZE if renormalize else 0, logits_type, scaling, logits_pitch,
                         _rows(logits, tokens, experts, logits_pitch, _float_bytes(logits_type, "logits_type"), "logits",
                               dev),
-                        _buffer(bias, experts * 4, "bias", dev), _buffer(token_count, 4, "token_count", dev),
-                        _buffer(weights, out, "weights", dev), _buffer(ids, out, "ids", dev))
+                        _buffer(bias, experts * 4, "bias", dev, 4), _buffer(token_count, 4, "token_count", dev, 4),
+                        _buffer(weights, out, "weights", dev, 4), _buffer(ids, out, "ids", dev, 4))
     _enqueue("cb200_moe_route", args, dev, stream)
 
 
@@ -615,19 +631,22 @@ def moe_dispatch(x, ids, weights, group_list, position, tokens, experts, top_k, 
     (row of each pair, -1 when dropped), row_index / row_weight [tokens * top_k], and x [tokens][k] written to its rows
     of q / scale in the format `fmt`.  workspace: moe_dispatch_workspace_size bytes."""
     dev = _device(ids, "ids")
+    _sizes(tokens | experts | top_k | k | x_pitch, tokens, experts, top_k, k, x_pitch)
     rows = tokens * top_k
     x_bytes = _float_bytes(x_type, "x_type")
     q_bytes, scale_bytes = _dispatch_sizes(rows, k, fmt, x_bytes)
     index_bytes = 8 if row_index_type == GROUP_LIST_INT64 else 4
+    list_bytes = 8 if group_list_type == GROUP_LIST_INT64 else 4
     args = MoeDispatchArgs(
         tokens, experts, top_k, k, fmt, x_type, expert_begin, group_list_type, group_list_kind, row_index_type, x_pitch,
         None if fmt == DISPATCH_INDEX else _rows(x, tokens, k, x_pitch, x_bytes, "x", dev),
-        _buffer(ids, rows * 4, "ids", dev), _buffer(weights, rows * 4, "weights", dev),
+        _buffer(ids, rows * 4, "ids", dev, 4), _buffer(weights, rows * 4, "weights", dev, 4),
         _buffer(tensor_scale, 4, "tensor_scale", dev), _buffer(q, q_bytes, "q", dev),
         _buffer(scale, scale_bytes, "scale", dev),
-        _buffer(group_list, experts * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", dev),
-        _buffer(position, rows * 4, "position", dev), _buffer(row_index, rows * index_bytes, "row_index", dev),
-        _buffer(row_weight, rows * 4, "row_weight", dev), _buffer(workspace, 0, "workspace", dev),
+        _buffer(group_list, experts * list_bytes, "group_list", dev, list_bytes),
+        _buffer(position, rows * 4, "position", dev, 4),
+        _buffer(row_index, rows * index_bytes, "row_index", dev, index_bytes),
+        _buffer(row_weight, rows * 4, "row_weight", dev, 4), _buffer(workspace, 0, "workspace", dev),
         0 if workspace is None else workspace.nbytes)
     _enqueue("cb200_moe_dispatch", args, dev, stream)
 
@@ -638,12 +657,15 @@ def moe_combine(d, position, weights, out, tokens, n, top_k, rows=None, d_type=D
     unless given), slots with a negative position skipped."""
     dev = _device(d, "d")
     rows = tokens * top_k if rows is None else rows
-    out_bytes = tokens * n * _float_bytes(out_type, "out_type")
+    _sizes(tokens | n | top_k | rows, tokens, n, top_k, rows)
+    d_elem, out_elem = _float_bytes(d_type, "d_type"), _float_bytes(out_type, "out_type")
+    out_bytes = tokens * n * out_elem
     args = MoeCombineArgs(tokens, top_k, n, rows, d_type, out_type, shared_weight, 0,
-                          _buffer(d, rows * n * _float_bytes(d_type, "d_type"), "d", dev),
-                          _buffer(position, tokens * top_k * 4, "position", dev),
-                          _buffer(weights, tokens * top_k * 4, "weights", dev), _buffer(shared, out_bytes, "shared", dev),
-                          _buffer(out, out_bytes, "out", dev))
+                          _buffer(d, rows * n * d_elem, "d", dev, d_elem),
+                          _buffer(position, tokens * top_k * 4, "position", dev, 4),
+                          _buffer(weights, tokens * top_k * 4, "weights", dev, 4),
+                          _buffer(shared, out_bytes, "shared", dev, out_elem),
+                          _buffer(out, out_bytes, "out", dev, out_elem))
     _enqueue("cb200_moe_combine", args, dev, stream)
 
 
@@ -657,13 +679,15 @@ def nvfp4_quantize(x, q, scale, rows, k, tensor_scale, x_type=DTYPE_BF16, x_pitc
     """x [rows][k] (with swiglu [rows][2k]: act next to gate) -> q [rows][k/2] bytes and E4M3 scales by rows ([rows][k/16]
     bytes) or tiled (nvfp4_tiled_scale_bytes bytes), in units of the device scalar tensor_scale."""
     dev = _device(x, "x")
+    _sizes(rows | k | x_pitch, rows, k, x_pitch)
     width = 2 * k if swiglu else k
+    count_bytes = 8 if row_count_type == GROUP_LIST_INT64 else 4
     scale_bytes = nvfp4_tiled_scale_bytes(rows, k) if scale_layout == NVFP4_SCALES_TILED else rows * (k // 16)
     args = Nvfp4QuantizeArgs(
         rows, k, x_type, scale_layout, NVFP4_SWIGLU if swiglu else 0, row_count_type, x_pitch,
         _rows(x, rows, width, x_pitch, _float_bytes(x_type, "x_type"), "x", dev),
         _buffer(tensor_scale, 4, "tensor_scale", dev),
-        _buffer(row_count, 8 if row_count_type == GROUP_LIST_INT64 else 4, "row_count", dev),
+        _buffer(row_count, count_bytes, "row_count", dev, count_bytes),
         _buffer(q, rows * (k // 2), "q", dev), _buffer(scale, scale_bytes, "scale", dev))
     _enqueue("cb200_nvfp4_quantize", args, dev, stream)
 
@@ -683,11 +707,13 @@ def nvfp4_matmul(a, b, scale_a, scale_b, d, m, n, k, workspace=None, alpha=None,
     """a [m][k/2], b [n][k/2] packed E2M1 with E4M3 scales by rows or tiled -> d [m][n] = alpha * a @ b^T.  alpha: device
     scalar (the product of the tensor scales); workspace: nvfp4_matmul_workspace_size bytes."""
     dev = _device(a, "a")
+    _sizes(m | n | k | block_num, m, n, k, block_num)
+    elem = _float_bytes(d_type, "d_type")
     args = Nvfp4MatmulArgs(
         m, n, k, scale_a_layout, scale_b_layout, d_type, _buffer(a, m * (k // 2), "a", dev), _buffer(b, n * (k // 2), "b", dev),
         _buffer(scale_a, _nvfp4_scale_bytes(m, k, scale_a_layout), "scale_a", dev),
-        _buffer(scale_b, _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", dev), _buffer(alpha, 4, "alpha", dev),
-        _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", dev), _buffer(workspace, 0, "workspace", dev),
+        _buffer(scale_b, _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", dev), _buffer(alpha, 4, "alpha", dev, 4),
+        _buffer(d, m * n * elem, "d", dev, elem), _buffer(workspace, 0, "workspace", dev),
         0 if workspace is None else workspace.nbytes, block_num, 0)
     _enqueue("cb200_nvfp4_matmul", args, dev, stream)
 
@@ -705,12 +731,15 @@ def nvfp4_grouped_matmul(a, b, group_list, scale_a, scale_b, d, m, n, k, group_c
     """Grouped slice-M NVFP4 matmul: a [m][k/2], b [G][n][k/2], scale_a by rows, scale_b by rows or tiled per group,
     alpha [G] on the device; rows past the last group are not written."""
     dev = _device(a, "a")
+    _sizes(m | n | k | group_count | block_num, m, n, k, group_count, block_num)
+    elem = _float_bytes(d_type, "d_type")
+    list_bytes = 8 if group_list_type == GROUP_LIST_INT64 else 4
     args = Nvfp4GroupedMatmulArgs(
         m, n, k, group_count, scale_b_layout, group_list_type, group_list_kind, d_type, _buffer(a, m * (k // 2), "a", dev),
         _buffer(b, group_count * n * (k // 2), "b", dev),
-        _buffer(group_list, group_count * (8 if group_list_type == GROUP_LIST_INT64 else 4), "group_list", dev),
+        _buffer(group_list, group_count * list_bytes, "group_list", dev, list_bytes),
         _buffer(scale_a, m * (k // 16), "scale_a", dev),
         _buffer(scale_b, group_count * _nvfp4_scale_bytes(n, k, scale_b_layout), "scale_b", dev),
-        _buffer(alpha, group_count * 4, "alpha", dev), _buffer(d, m * n * _float_bytes(d_type, "d_type"), "d", dev),
+        _buffer(alpha, group_count * 4, "alpha", dev, 4), _buffer(d, m * n * elem, "d", dev, elem),
         _buffer(workspace, 0, "workspace", dev), 0 if workspace is None else workspace.nbytes, block_num, 0)
     _enqueue("cb200_nvfp4_grouped_matmul_slice_m", args, dev, stream)

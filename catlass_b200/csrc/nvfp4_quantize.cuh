@@ -167,8 +167,9 @@ struct Raw16 {
     }
 };
 
-// The next block's loads are in flight while a block is worked on.  A thread's blocks are gridDim * 256 apart; (row, block) advance by that step without a division.  Four neighbouring
-// lanes hold the four bytes of a scale word where a row has whole words (p.word_stores): one of them stores it.
+// The next block's loads are in flight while a block is worked on.  A thread's blocks are gridDim * 256 apart; (row,
+// block) advance by that step without a division.  Four neighbouring lanes hold the four bytes of a scale word where a
+// row has whole words (p.word_stores): one of them stores it.
 template <int kType, bool kSwiglu>
 __global__ void __launch_bounds__(kNvQuantThreads, nv_quant_ctas(kType, kSwiglu))
 nvfp4_quantize_kernel(const NvQuantParams p)

@@ -679,8 +679,8 @@ CB200_API int cb200_moe_dispatch(const cb200_moe_dispatch_args *args, void *stre
  * Combine: the weighted sum of a token's expert rows, for grouped matmuls that write D row by row (W8A8, MX, NVFP4;
  * cb200_mx_grouped_matmul_finalize_routing has it fused):
  *     out[t] = round( shared_weight * shared[t] + sum_j weights[t][j] * d[position[t][j]] )       fp32, j ascending
- * Slots with position < 0 or >= rows are skipped (their weight is not read into the sum); shared may be NULL.  Every
- * row of out is written, with the same bits on every run.  No workspace.
+ * Slots with position < 0 or >= rows are skipped (their weight is not read into the sum); shared may be NULL, or out
+ * itself.  Every row of out is written, with the same bits on every run.  No workspace.
  */
 typedef struct cb200_moe_combine_args {
     uint32_t tokens;
@@ -771,7 +771,7 @@ typedef struct cb200_nvfp4_matmul_args {
     void *d;
     void *workspace;
     uint64_t workspace_bytes;
-    uint32_t block_num;           /* upper bound on the CTAs launched; 0 = one per SM */
+    uint32_t block_num;           /* upper bound on the CTAs launched (two at least); 0 = one per SM */
     uint32_t flags;               /* 0 */
 } cb200_nvfp4_matmul_args;
 

@@ -197,6 +197,23 @@ def test_python_calls_check_their_tensors(capi):
         capi.nvfp4_quantize(t, t, t, 4, 64, t)
 
 
+def test_python_calls_refuse_sizes_and_element_types(capi):
+    """Sizes that a 32-bit field would wrap, and tensors whose elements are not of the size the kernel reads."""
+    torch = pytest.importorskip("torch")
+    for bad in ((-1, 4), (4, 1 << 31), ((1 << 32) + 4, 4)):
+        with pytest.raises(ValueError):
+            capi._sizes(bad[0] | bad[1], *bad)
+    capi._sizes(0 | ((1 << 31) - 1), 0, (1 << 31) - 1)
+    ids = torch.zeros((8,), dtype=torch.int64)
+    here = ids.get_device()
+    with pytest.raises(ValueError):
+        capi._buffer(ids, 32, "ids", here, 4)
+    assert capi._buffer(ids.to(torch.int32), 32, "ids", here, 4) != 0
+    assert capi._buffer(ids.view(torch.uint8), 32, "ids", here, 4) == ids.data_ptr()    # raw bytes
+    with pytest.raises(ValueError):
+        capi._rows(torch.zeros((4, 16)), 4, 16, 16, 2, "x", here)
+
+
 def test_reference_rounding():
     """The plain definitions themselves: ties of both small formats, and a scale that lands on the largest value."""
     assert list(R.E2M1[R.nearest_even(np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 99.0]), R.E2M1)]) == \

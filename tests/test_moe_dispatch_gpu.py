@@ -228,3 +228,31 @@ def test_combine_refuses_and_skips(cuda):
         capi.moe_combine(d, position, w, out, 2, 16, 2, rows=5, d_type=0, out_type=0)
     with pytest.raises(ValueError):
         capi.moe_combine(d, position, w, out, 3, 16, 2, rows=4, d_type=0, out_type=0)
+
+
+def test_int64_ids_are_refused(cuda):
+    import torch
+    from catlass_b200 import capi
+    ids = torch.zeros((16, 2), dtype=torch.int64, device=cuda)
+    position, gl = torch.empty((16, 2), dtype=torch.int32, device=cuda), torch.empty((8,), dtype=torch.int64, device=cuda)
+    with pytest.raises(ValueError, match="elements of 4 bytes"):
+        capi.moe_dispatch(None, ids, None, gl, position, 16, 8, 2, 0, capi.DISPATCH_INDEX)
+    x = torch.zeros((16, 64), device=cuda)
+    q = torch.empty((32, 64), dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError, match="x must have"):    # fp32 rows under the default type code, bf16
+        capi.moe_dispatch(x, ids.to(torch.int32), None, gl, position, 16, 8, 2, 64, capi.DISPATCH_COPY, q=q)
+
+
+@pytest.mark.parametrize("n", [7, 514, 4096])
+def test_combine_onto_the_shared_rows(cuda, n):
+    """out may be shared itself: every element is read by the thread that writes it.  Small integers: exact sums."""
+    import torch
+    from catlass_b200 import capi
+    g = torch.Generator(device="cpu").manual_seed(n)
+    d = torch.randint(-4, 5, (40, n), generator=g).to(torch.bfloat16).to(cuda)
+    shared = torch.randint(-4, 5, (20, n), generator=g).to(torch.bfloat16).to(cuda)
+    position = torch.randperm(40, generator=g).view(20, 2).to(torch.int32).to(cuda)
+    w = torch.randint(1, 3, (20, 2), generator=g).float().to(cuda)
+    want = shared.float() + (w[:, :, None] * d.float()[position.long()]).sum(1)
+    capi.moe_combine(d, position, w, shared, 20, n, 2, shared=shared)
+    assert torch.equal(shared.float(), want)
