@@ -586,6 +586,7 @@ CB200_API int cb200_quantize_per_token_int8(const cb200_quantize_int8_args *args
  *              CB200_ROUTE_RENORMALIZE (a sum of zero gives zeros), times `scaling`
  * Ties, of experts and of runs, go to the lower index.  The order is that of the exact keys: where two keys are closer
  * than 32-bit arithmetic can tell apart, they are worked out again in 64 bits.
+ * (Two runs whose sums of two different keys agree to the last bits of those 64 may come in either order.)
  * An expert whose logit is -inf or NaN cannot be chosen and has s = 0; slots left without an expert get id -1 and
  * weight 0, which cb200_moe_dispatch and cb200_moe_combine skip.  Logits of +inf share the softmax among themselves.
  * token_count (optional, device, int32): tokens at or beyond it (a padded batch) get ids -1 and weights 0.
